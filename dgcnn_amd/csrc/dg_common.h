@@ -326,6 +326,11 @@ __device__ __forceinline__ void dg_adam_elem(float g, float m, float v, float p,
   mo = mi; vo = vi;
   po = __builtin_fmaf(-lr_over_bc1, mi / denom, p);
 }
+// a batch's mean loss into the running sum: product and sum rounded apart, in every kernel that keeps the metrics
+__device__ __forceinline__ float dg_add_scaled(float sum, float loss, float scale) {
+#pragma clang fp contract(off)
+  return sum + loss * scale;
+}
 // workgroup barrier that orders LDS traffic only: outstanding GLOBAL stores/loads are NOT drained
 // (a plain __syncthreads() waits vmcnt(0), i.e. a full HBM write round trip per barrier)
 #ifdef DG_EMU

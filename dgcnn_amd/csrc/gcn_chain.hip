@@ -1783,7 +1783,7 @@ k_chain_readout_eval(int N, int B, int F, const int* __restrict__ graph_ptr, con
   sl[0] += sl[2]; sl[1] += sl[3]; sc[0] += sc[2]; sc[1] += sc[3];      // st = 128
   sl[0] += sl[1]; sc[0] += sc[1];                                      // st = 64
   for (int st = 32; st >= 1; st >>= 1) { sl[0] += __shfl_down(sl[0], st); sc[0] += __shfl_down(sc[0], st); }
-  if (lane == 0) { t.metrics[0] += sl[0] * t.scale; t.metrics[1] += sc[0]; }
+  if (lane == 0) { t.metrics[0] = dg_add_scaled(t.metrics[0], sl[0], t.scale); t.metrics[1] += sc[0]; }
 }
 
 // =================================================================================================================

@@ -838,7 +838,7 @@ k_eval_metrics(int B, int C, const float* __restrict__ logp, const int64_t* __re
     if ((int)threadIdx.x < st) { sl[threadIdx.x] += sl[threadIdx.x + st]; sc[threadIdx.x] += sc[threadIdx.x + st]; }
     __syncthreads();
   }
-  if (threadIdx.x == 0) { metrics[0] += sl[0] * scale; metrics[1] += sc[0]; }
+  if (threadIdx.x == 0) { metrics[0] = dg_add_scaled(metrics[0], sl[0], scale); metrics[1] += sc[0]; }
 }
 
 int dg_launch_eval_metrics(int B, int C, const float* logp, const int64_t* y, float* metrics, float loss_scale, hipStream_t s) {
