@@ -22,6 +22,7 @@ There is NO CPU/eager fallback: on a CPU tensor, or without ``libdgcnn_hip.so``,
 """
 from __future__ import annotations
 
+import itertools
 import math
 from typing import List, Optional
 
@@ -77,6 +78,9 @@ def _batch_size_of(data) -> int:
     return int(B)
 
 
+# Every model's forward tags start somewhere else in the 31-bit range: a workspace is uninitialised memory, and an error word that another
+# model's batch left there must not read as one of this model's.
+_MODELS = itertools.count()
 _WS_BYTES = {}      # (N, E, B, F, C) -> dgcnn_workspace_bytes: a pure function of the dimensions, memoised (one ctypes call per step otherwise)
 
 
@@ -166,7 +170,7 @@ class Model(nn.Module):
         self._last_ws = None
         self._last_dims = None
         self._last_flat_grad = None
-        self._epoch = 0
+        self._epoch = next(_MODELS) * 0x9E3779B1 % 0x7FFFFFFE
 
     # ---- flat parameter buffer ---------------------------------------------------------
     def _param_list(self) -> List[nn.Parameter]:

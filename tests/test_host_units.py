@@ -137,3 +137,14 @@ def test_data_can_restrict_its_own_forms():
     fl = m._flags_of(d)
     assert fl & _lib.FLAG_COALESCED_UNDIRECTED and fl & _lib.FLAG_AGG_SPARSE and fl & _lib.FLAG_NO_CHAIN
     assert _lib.lib().dgcnn_forward_form(3800, 140000, 50, 1, fl, 180) == 0          # CSR gather kernels, whatever the sizes admit
+
+
+def test_forward_tags_of_two_models_do_not_meet():
+    """an uninitialised workspace may hold the error word that another model's batch left there: tags of different models lie far apart"""
+    from dgcnn_amd.model import Model
+    starts = [Model(3, 2)._epoch for _ in range(64)]
+    gaps = [abs(a - b) for i, a in enumerate(starts) for b in starts[:i]]
+    assert min(min(g, 0x7FFFFFFE - g) for g in gaps) > 1 << 20
+    m = Model(3, 2)
+    m.__dict__["_epoch"] = 0x7FFFFFFE
+    assert m._next_epoch() == 1          # (never 0: a cleared word is no tag)
