@@ -9,12 +9,12 @@ from __future__ import annotations
 import ctypes
 import os
 import subprocess
-from ctypes import c_char_p, c_float, c_int, c_int64, c_uint64, c_void_p
+from ctypes import c_char_p, c_double, c_float, c_int, c_int64, c_uint64, c_void_p
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("DGCNN_HIP_LIB") or os.path.join(_HERE, "libdgcnn_hip.so")   # env override: A/B experiments
 CSRC = os.path.join(_HERE, "csrc")
-ABI_VERSION = 20
+ABI_VERSION = 21
 FLAG_COALESCED_UNDIRECTED = 1
 FLAG_FORCE_FUSED = 2
 FLAG_FORCE_TILED = 4
@@ -27,6 +27,7 @@ FLAG_EXCLUSIVE_DEVICE = 512   # pipelined steps: nothing else runs on this devic
 FLAG_INFERENCE = 1024     # forward-only use of the batch: one-launch evaluation kernel also for graphs of 257..512 nodes (ABI v20)
 FLAG_BF16 = 64            # bf16 leg: pre-scaled linear outputs stored bf16, X.W on the bf16 matrix cores
 
+F32, BF16, F16 = 0, 1, 2      # element types of the layer and optimizer operators
 FORM_DENSE, FORM_CHAIN, FORM_CHAIN_TAIL, FORM_STEP, FORM_EVAL = 1, 2, 4, 8, 16      # dgcnn_forward_form bits
 
 K = 30
@@ -59,6 +60,29 @@ class Dataset(ctypes.Structure):
     _fields_ = [("G", c_int64), ("Ntot", c_int64), ("Etot", c_int64), ("F", ctypes.c_int32), ("reserved_", ctypes.c_int32),
                 ("node_ptr", c_void_p), ("y", c_void_p), ("x", c_void_p), ("rowptr", c_void_p), ("colidx", c_void_p),
                 ("dinv", c_void_p), ("xs", c_void_p), ("adj_bits", c_void_p)]
+
+
+class AdamwTensor(ctypes.Structure):
+    """``dgcnn_adamw_tensor`` of include/dgcnn_hip.h"""
+    _fields_ = [("param", c_void_p), ("grad", c_void_p), ("exp_avg", c_void_p), ("exp_avg_sq", c_void_p), ("exp_avg_scale", c_void_p),
+                ("exp_avg_sq_scale", c_void_p), ("master", c_void_p), ("numel", c_int64)]
+
+
+class AdamwArgs(ctypes.Structure):
+    """``dgcnn_adamw_args`` of include/dgcnn_hip.h"""
+    _fields_ = [("lr", c_double), ("beta1", c_double), ("beta2", c_double), ("eps", c_double), ("weight_decay", c_double),
+                ("step", c_int64), ("step_dev", c_void_p), ("lr_dev", c_void_p), ("scalars_dev", c_void_p),
+                ("seed", c_uint64), ("first_index", c_int64),
+                ("param_dtype", ctypes.c_int32), ("grad_dtype", ctypes.c_int32), ("state_bits", ctypes.c_int32), ("count", ctypes.c_int32),
+                ("tensors", c_void_p)]
+
+
+class GroupNormArgs(ctypes.Structure):
+    """``dgcnn_group_norm_args`` of include/dgcnn_hip.h"""
+    _fields_ = [("rows", c_int64), ("channels", ctypes.c_int32), ("groups", ctypes.c_int32), ("segments", ctypes.c_int32),
+                ("dtype", ctypes.c_int32), ("weight_dtype", ctypes.c_int32), ("act", ctypes.c_int32), ("eps", c_float),
+                ("reserved_", ctypes.c_int32), ("x", c_void_p), ("weight", c_void_p), ("bias", c_void_p), ("ptr", c_void_p),
+                ("mean", c_void_p), ("rstd", c_void_p)]
 
 
 # name -> (restype, argtypes); must list every symbol include/dgcnn_hip.h declares
@@ -100,6 +124,10 @@ SIGNATURES = {
                                           c_void_p, c_int64, c_float, c_float, c_float, c_float, c_int, c_int, c_void_p]),
     "dgcnn_adam_step": (c_int, [c_void_p] * 4 + [c_int64, c_int64, c_float, c_float, c_float, c_float, c_int,
                                 c_void_p]),
+    "dgcnn_adamw_step": (c_int, [ctypes.POINTER(AdamwArgs), c_void_p]),
+    "dgcnn_group_norm_workspace_bytes": (c_int64, [c_int64] + [c_int] * 6),
+    "dgcnn_group_norm_fwd": (c_int, [ctypes.POINTER(GroupNormArgs)] + [c_void_p] * 3),
+    "dgcnn_group_norm_bwd": (c_int, [ctypes.POINTER(GroupNormArgs)] + [c_void_p] * 6),
     "dgcnn_collate": (c_int, [c_int, c_int, c_int64, c_int64, c_int64] + [c_void_p] * 13),
     "dgcnn_collate_ids": (c_int, [c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int64]
                           + [c_void_p] * 5 + [c_int64, c_int64] + [c_void_p] * 5 + [c_void_p]),
@@ -173,6 +201,13 @@ def lib() -> ctypes.CDLL:
 def check(rc: int, what: str) -> None:
     if rc != 0:
         raise DgcnnError(f"{what} failed: {_ERR.get(rc, rc)}")
+
+
+def checked_bytes(n: int, what: str) -> int:
+    """a size query's answer; a negative one is its error"""
+    if n < 0:
+        raise DgcnnError(f"{what} failed: {_ERR.get(n, n)}")
+    return int(n)
 
 
 def param_layout(F: int, C: int):

@@ -12,8 +12,16 @@ Semantics are those of ``torch.optim.Adam`` defaults (no weight decay, no amsgra
 per parameter in ``state_dict()``).  Whenever the flat layout is NOT recognised (other modules' parameters, gradients
 that are not views of one buffer, a parameter without gradient, ...) the step falls back to torch's own implementation
 for that call -- same numbers, just slower.  GPU tensors only take the fused route.
+
+:class:`AdamW` (decoupled weight decay) updates ANY list of GPU tensors with one launch for each 48 of them, through
+:func:`adamw_step`: fp32, bf16 and fp16 parameters, fp32 copies of 16-bit ones, moments in 32 or in 8 bits, captured steps.
 """
 from __future__ import annotations
+
+import contextlib
+import ctypes
+from itertools import chain
+from typing import Optional, Sequence, Union
 
 import torch
 from torch.optim import Optimizer
@@ -200,3 +208,203 @@ class Adam(Optimizer):
         _adam(with_grad, grads, ms, vs, [], steps, amsgrad=False, beta1=b1, beta2=b2, lr=group["lr"], weight_decay=0.0,
               eps=group["eps"], maximize=False, foreach=None, capturable=False, differentiable=False, fused=None,
               grad_scale=None, found_inf=None, has_complex=False)
+
+
+# ---- AdamW over many tensors -------------------------------------------------------------------------------------------------------------
+STATE_BLOCK = 256           # elements of a tensor that share one scale of an 8-bit moment
+_DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
+
+
+def _refuse(cond: bool, msg: str) -> None:
+    if cond:
+        raise _lib.DgcnnError(msg)
+
+
+def _capturing() -> bool:
+    return torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing()
+
+
+def _check_list(name, ts, params, dtypes, blocks=False) -> None:
+    _refuse(len(ts) != len(params), f"{name}: {len(ts)} tensors for {len(params)} parameters")
+    dev = params[0].device
+    for t, p in zip(ts, params):
+        n = -(-p.numel() // STATE_BLOCK) if blocks else p.numel()
+        if t.dtype not in dtypes or t.numel() != n or t.device != dev or not (t.is_contiguous() if blocks else t.stride() == p.stride()):
+            raise _lib.DgcnnError(f"{name}: a tensor is {tuple(t.shape)} {t.dtype} on {t.device} with strides {t.stride()}; its parameter is {tuple(p.shape)} "
+                                  f"{p.dtype} on {dev} with strides {p.stride()} (types here: {', '.join(map(str, dtypes))}"
+                                  + (f"; [ceil(numel / {STATE_BLOCK})] contiguous)" if blocks else "; the parameter's shape and strides)"))
+
+
+def _dense(p) -> bool:
+    return p.is_contiguous() or (p.dim() == 4 and p.is_contiguous(memory_format=torch.channels_last)) or \
+        (p.dim() == 5 and p.is_contiguous(memory_format=torch.channels_last_3d))
+
+
+def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], exp_avgs: Sequence[torch.Tensor], exp_avg_sqs: Sequence[torch.Tensor], *,
+               step: Union[int, torch.Tensor], lr: Union[float, torch.Tensor] = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2,
+               masters: Optional[Sequence[torch.Tensor]] = None, exp_avg_scales: Optional[Sequence[torch.Tensor]] = None,
+               exp_avg_sq_scales: Optional[Sequence[torch.Tensor]] = None, seed: int = 0) -> None:
+    """One AdamW step over lists of tensors on one device, in place, without synchronising::
+
+        m = b1 m + (1 - b1) g      v = b2 v + (1 - b2) g^2      p = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+
+    ``params`` are of one type (float32, bfloat16, float16), dense, and no two of them share memory; ``grads`` of the same type, or float32.
+    Moments are float32, or -- with both scale lists -- 8 bits: ``exp_avgs`` and ``exp_avg_sqs`` then are ``torch.float8_e4m3fn`` codes of ``m`` and of
+    ``sqrt(v)``, each times one float32 scale for 256 consecutive elements (``[ceil(numel / 256)]``).  Codes are rounded stochastically by a hash of
+    (``seed``, tensor, step, element), so that the means do not stall between two codes; equal arguments give equal bits.
+    ``masters``: float32 copies of 16-bit parameters, which are what is updated; the parameters get the rounded values.
+
+    ``step`` is this step's number, from 1 on.  For a step captured into a graph, ``step`` is an int64 device tensor of one element that holds the steps done
+    so far (each replay counts it up), and ``lr`` may be a float32 device tensor of one element."""
+    if len(params) == 0:
+        return
+    p0 = params[0]
+    dev = p0.device
+    _refuse(not p0.is_cuda, "dgcnn_amd.optim.adamw_step runs only on an AMD GPU through libdgcnn_hip.so; got a CPU tensor")
+    _refuse(p0.dtype not in _DTYPES, f"parameters must be float32, bfloat16 or float16, got {p0.dtype}")
+    for p in params:
+        if p.dtype != p0.dtype or p.device != dev or not _dense(p):
+            raise _lib.DgcnnError(f"parameters must be dense tensors of one type on one device: got {p0.dtype} on {dev} and {p.dtype} on {p.device} "
+                                  f"{tuple(p.shape)} with strides {p.stride()}")
+    bits = 32 if exp_avg_scales is None else 8
+    _refuse((exp_avg_scales is None) != (exp_avg_sq_scales is None), "8-bit moments need both exp_avg_scales and exp_avg_sq_scales")
+    _refuse(len(grads) != len(params), f"grads: {len(grads)} tensors for {len(params)} parameters")
+    g0 = grads[0].dtype
+    _check_list("grads", grads, params, (p0.dtype,) if g0 == p0.dtype else (torch.float32,))
+    state = (torch.float32,) if bits == 32 else (torch.float8_e4m3fn,)
+    _check_list("exp_avgs", exp_avgs, params, state)
+    _check_list("exp_avg_sqs", exp_avg_sqs, params, state)
+    lists = [params, grads, exp_avgs, exp_avg_sqs]
+    for name, ts in (("exp_avg_scales", exp_avg_scales), ("exp_avg_sq_scales", exp_avg_sq_scales)):
+        if ts is not None:
+            _check_list(name, ts, params, (torch.float32,), blocks=True)
+    if masters is not None:
+        _refuse(p0.dtype == torch.float32, "masters are for bfloat16 and float16 parameters")
+        _check_list("masters", masters, params, (torch.float32,))
+    _refuse(not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0), f"betas must lie in [0, 1), got {betas}")
+    _refuse(not eps >= 0.0, f"eps must not be negative, got {eps}")
+
+    a = _lib.AdamwArgs()
+    keep = None
+    if isinstance(step, torch.Tensor):
+        _refuse(step.dtype != torch.int64 or step.numel() != 1 or step.device != dev, f"step must be an int or an int64 tensor of one element on {dev}")
+        keep = torch.empty(16, dtype=torch.float32, device=dev)
+        a.step_dev, a.scalars_dev = step.data_ptr(), keep.data_ptr()
+        if isinstance(lr, torch.Tensor):
+            _refuse(lr.dtype != torch.float32 or lr.numel() != 1 or lr.device != dev, f"lr must be a float or a float32 tensor of one element on {dev}")
+            a.lr_dev, lr = lr.data_ptr(), 0.0
+    else:
+        _refuse(step < 1, f"step counts from 1, got {step}")
+        _refuse(isinstance(lr, torch.Tensor), "lr may be a tensor only where step is one")
+        _refuse(_capturing(), "a captured step needs its counter on the device: step as an int64 tensor (AdamW: capturable=True)")
+        a.step = step
+    a.lr, a.beta1, a.beta2, a.eps, a.weight_decay = lr, betas[0], betas[1], eps, weight_decay
+    a.seed, a.first_index = seed & 0xFFFFFFFFFFFFFFFF, 0
+    a.param_dtype, a.grad_dtype, a.state_bits, a.count = _DTYPES[p0.dtype], _DTYPES[g0], bits, len(params)
+    none = [0] * len(params)
+    at = lambda ts: none if ts is None else [t.data_ptr() for t in ts]      # noqa: E731
+    where = at(params)
+    _refuse(len(set(where)) < sum(1 for p in params if p.numel()), "a parameter is in the list twice")
+    columns = [where, at(grads), at(exp_avgs), at(exp_avg_sqs), at(exp_avg_scales), at(exp_avg_sq_scales), at(masters), [p.numel() for p in params]]
+    table = (ctypes.c_int64 * (8 * len(params)))(*chain.from_iterable(zip(*columns)))
+    a.tensors = ctypes.addressof(table)
+    with contextlib.nullcontext() if dev.index is None or dev.index == torch.cuda.current_device() else torch.cuda.device(dev):
+        _lib.check(_lib.lib().dgcnn_adamw_step(ctypes.byref(a), torch.cuda.current_stream(dev).cuda_stream), "dgcnn_adamw_step")
+
+
+class AdamW(Optimizer):
+    """``torch.optim.AdamW`` (no amsgrad) over GPU parameters of any layout: one launch for each 48 tensors of a type.
+
+    ``state_bits`` 32: float32 moments, ``state_dict()`` as torch's (and torch's loads).  8: moments as :func:`adamw_step` describes them, a quarter of
+    the bytes; the state then holds ``exp_avg``, ``exp_avg_sq`` (codes of the mean and of the root of the mean square) and their ``_scale`` tensors.
+    ``master_weights``: bfloat16 / float16 parameters get a float32 copy (``master`` in the state) that carries the updates too small for their type.
+    ``capturable``: the step counter lives on the device and ``step()`` may be captured into a graph; ``lr`` may then be a float32 device tensor of one
+    element.  A parameter without a gradient is left alone; ``seed`` picks the random rounding of 8-bit moments."""
+
+    def __init__(self, params, lr: Union[float, torch.Tensor] = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2, amsgrad: bool = False, *,
+                 state_bits: int = 32, master_weights: bool = False, capturable: bool = False, seed: int = 0):
+        if amsgrad:
+            raise ValueError("dgcnn_amd.optim.AdamW has no amsgrad variant; use torch.optim.AdamW")
+        if state_bits not in (8, 32):
+            raise ValueError(f"state_bits must be 8 or 32, got {state_bits}")
+        if not isinstance(lr, torch.Tensor) and not lr >= 0.0:
+            raise ValueError(f"lr must not be negative, got {lr}")
+        if isinstance(lr, torch.Tensor) and not capturable:
+            raise ValueError("lr may be a tensor only with capturable=True")
+        if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0) or not eps >= 0.0 or not weight_decay >= 0.0:
+            raise ValueError(f"betas must lie in [0, 1), eps and weight_decay must not be negative: got {betas}, {eps}, {weight_decay}")
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits, master_weights=master_weights,
+                                      capturable=capturable, seed=seed))
+
+    def _state_of(self, p, group, fresh):
+        st = self.state[p]
+        if not st:
+            _refuse(_capturing(), "run a step() before capturing one: the state would be set up anew by every replay")
+            # (tensors that start together share their counter: they can go into one call)
+            st["step"] = fresh.setdefault(p.device, torch.zeros(1, dtype=torch.int64, device=p.device)) if group["capturable"] else 0
+            if group["state_bits"] == 32:
+                st["exp_avg"], st["exp_avg_sq"] = (torch.zeros_like(p, dtype=torch.float32, memory_format=torch.preserve_format) for _ in range(2))
+            else:
+                for k in ("exp_avg", "exp_avg_sq"):
+                    st[k] = torch.zeros_like(p, dtype=torch.uint8, memory_format=torch.preserve_format).view(torch.float8_e4m3fn)
+                    st[k + "_scale"] = torch.zeros(-(-p.numel() // STATE_BLOCK), dtype=torch.float32, device=p.device)
+        if group["master_weights"] and p.dtype != torch.float32 and "master" not in st:
+            st["master"] = p.detach().to(torch.float32, copy=True)
+        t = st["step"]
+        if group["capturable"] != isinstance(t, torch.Tensor) or (group["capturable"] and (t.dtype != torch.int64 or t.device != p.device)):
+            n = int(t)              # (a state of another kind was loaded: torch's counters are float32 tensors)
+            st["step"] = fresh.setdefault((p.device, n), torch.full((1,), n, dtype=torch.int64, device=p.device)) if group["capturable"] else n
+        return st
+
+    def load_state_dict(self, state_dict) -> None:
+        """As ``Optimizer.load_state_dict``, but every tensor of the state keeps its own type (torch's casts them to the parameter's, which codes, scales
+        and the float32 moments of 16-bit parameters do not survive)."""
+        super().load_state_dict(state_dict)
+        saved = list(chain.from_iterable(g["params"] for g in state_dict["param_groups"]))
+        mine = list(chain.from_iterable(g["params"] for g in self.param_groups))
+        for k, p in zip(saved, mine):
+            for name, v in state_dict["state"].get(k, {}).items():
+                if isinstance(v, torch.Tensor):
+                    # (counters come back as host numbers: step() makes one device counter for all equal ones)
+                    self.state[p][name] = int(v) if name == "step" else v.detach().to(p.device, copy=True)
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for group in self.param_groups:
+            calls, fresh = {}, {}
+            for p in group["params"]:
+                g = p.grad
+                if g is None:
+                    continue
+                _refuse(g.is_sparse, "dgcnn_amd.optim.AdamW takes dense gradients")
+                if g.stride() != p.stride() and _dense(p):
+                    g = torch.empty_like(p, dtype=g.dtype).copy_(g)
+                st = self._state_of(p, group, fresh)
+                t = st["step"]
+                calls.setdefault((p.device, p.dtype, g.dtype, "master" in st, t.data_ptr() if group["capturable"] else t), []).append((p, g, st))
+            if group["capturable"]:
+                counted = set()
+                for items in calls.values():      # a call counts its counter up: no two calls may share one
+                    t = items[0][2]["step"]
+                    if t.data_ptr() in counted:
+                        _refuse(_capturing(), "run a step() with these gradients' types before capturing one")
+                        t = t.clone()
+                        for _, _, st in items:
+                            st["step"] = t
+                    counted.add(t.data_ptr())
+            for key, items in calls.items():
+                ps, gs, sts = zip(*items)
+                t = sts[0]["step"] if group["capturable"] else sts[0]["step"] + 1
+                more = {k + "s": [st[k] for st in sts] for k in ("exp_avg_scale", "exp_avg_sq_scale") if k in sts[0]}
+                if key[3]:
+                    more["masters"] = [st["master"] for st in sts]
+                adamw_step(ps, gs, [st["exp_avg"] for st in sts], [st["exp_avg_sq"] for st in sts], step=t, lr=group["lr"], betas=group["betas"],
+                           eps=group["eps"], weight_decay=group["weight_decay"], seed=group["seed"], **more)
+                if not group["capturable"]:
+                    for st in sts:
+                        st["step"] = t
+        return loss

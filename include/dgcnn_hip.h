@@ -32,7 +32,7 @@
 extern "C" {
 #endif
 
-#define DGCNN_ABI_VERSION 20
+#define DGCNN_ABI_VERSION 21
 
 /* error codes */
 #define DGCNN_OK            0
@@ -337,6 +337,65 @@ int dgcnn_model_backward_step(int N, int E, int B, int F, int C, float* params, 
 int dgcnn_adam_step(float* params, float* grads, float* exp_avg, float* exp_avg_sq,
                     int64_t n, int64_t step, float lr, float beta1, float beta2, float eps,
                     int zero_grads, dgcnn_stream_t stream);
+
+/* ------------------------------------------------------------------------------------
+ * (ABI v21) Operators of wider networks on the same batches: products grouped by type, group norm with an activation, AdamW over many
+ * tensors.  Element types are run-time values; sums, statistics and moments are fp32, every result is rounded to its type once.
+ * ---------------------------------------------------------------------------------- */
+#define DGCNN_F32  0
+#define DGCNN_BF16 1
+#define DGCNN_F16  2
+
+/* AdamW (decoupled weight decay) over `count` tensors in one launch for each 48 of them:
+ *   m = b1 m + (1-b1) g;  v = b2 v + (1-b2) g^2;  p = p (1 - lr wd) - lr/(1-b1^t) m / (sqrt(v)/sqrt(1-b2^t) + eps)
+ * A tensor is `numel` dense elements of param_dtype; grad is of grad_dtype: the same, or fp32.
+ * state_bits 32: exp_avg = m, exp_avg_sq = v, fp32.  state_bits 8: exp_avg and exp_avg_sq hold e4m3 codes of m and of sqrt(v), with one fp32
+ * scale for each 256 consecutive elements in exp_avg_scale / exp_avg_sq_scale [ceil(numel/256)]: value = code * scale.  Codes are rounded
+ * stochastically from a hash of (seed, first_index + tensor, step, element): equal arguments give equal bits.
+ * master (fp32, for 16-bit parameters; all tensors of a call or none): the parameter's full-precision copy, which is what is updated; param
+ * gets its rounded value.
+ * step >= 1 is this step's number; or step_dev points to a device counter of the steps done so far, which the call increments (for
+ * captured steps; scalars_dev: 16 floats of device scratch; lr_dev: the learning rate on the device, or NULL for lr).
+ * Tensors with numel 0 are skipped; no two tensors may overlap.  Pointers of `tensors` are read during the call only. */
+typedef struct dgcnn_adamw_tensor {
+  void* param; const void* grad; void* exp_avg; void* exp_avg_sq;
+  float* exp_avg_scale; float* exp_avg_sq_scale; float* master;
+  int64_t numel;
+} dgcnn_adamw_tensor;
+typedef struct dgcnn_adamw_args {
+  double lr, beta1, beta2, eps, weight_decay;
+  int64_t step; int64_t* step_dev; const float* lr_dev; float* scalars_dev;
+  uint64_t seed; int64_t first_index;
+  int32_t param_dtype, grad_dtype, state_bits, count;
+  const dgcnn_adamw_tensor* tensors;      /* host */
+} dgcnn_adamw_args;
+int dgcnn_adamw_step(const dgcnn_adamw_args* args, dgcnn_stream_t stream);
+
+/* Group norm with an activation over rows of channels [rows, channels] (row-major, channels last), statistics for each segment of rows and each
+ * group of channels / groups channels:  y = act((x - mean) / sqrt(var + eps) * weight + bias), var the mean squared difference.
+ * ptr [segments + 1] int64 (device, ascending): segment s is rows ptr[s] .. ptr[s+1]-1, e.g. a batch's graphs; rows outside are set to
+ * 0 in y and dx; a segment may be empty.  ptr NULL: `segments` samples of rows / segments rows each.  (A ptr that does not ascend, or points
+ * outside [0, rows], gives unspecified values, never an access outside the tensors.)  segments 0: y and dx are not written.
+ * weight, bias [channels] of weight_dtype, each may be NULL (1 and 0).  mean, rstd [segments, groups] fp32: written by _fwd, read by _bwd.
+ * x, y, dy, dx are of dtype; dweight and dbias (each may be NULL) of weight_dtype.  Channels of a group: at most 1024 in
+ * any case, 2048 if fp32 and a multiple of 4, 4096 if 16-bit and a multiple of 8 (tensors 16-byte aligned), else DGCNN_EUNSUPPORTED.
+ * ws: dgcnn_group_norm_workspace_bytes(rows, channels, groups, segments, ptr == NULL, dtype, backward) bytes. */
+#define DGCNN_ACT_NONE 0
+#define DGCNN_ACT_RELU 1
+#define DGCNN_ACT_SILU 2
+#define DGCNN_ACT_GELU 3      /* z * (1 + erf(z / sqrt 2)) / 2 */
+#define DGCNN_ACT_TANH 4
+typedef struct dgcnn_group_norm_args {
+  int64_t rows;
+  int32_t channels, groups, segments, dtype, weight_dtype, act;
+  float eps; int32_t reserved_;
+  const void* x; const void* weight; const void* bias; const int64_t* ptr;
+  float* mean; float* rstd;
+} dgcnn_group_norm_args;
+int64_t dgcnn_group_norm_workspace_bytes(int64_t rows, int channels, int groups, int segments, int dense, int dtype, int backward);
+int dgcnn_group_norm_fwd(const dgcnn_group_norm_args* args, void* y, void* ws, dgcnn_stream_t stream);
+int dgcnn_group_norm_bwd(const dgcnn_group_norm_args* args, const void* dy, void* dx, void* dweight, void* dbias, void* ws,
+                         dgcnn_stream_t stream);
 
 /* ------------------------------------------------------------------------------------
  * Pipelined training step: the body of the reference's `train()` loop (/root/reference/train.py:36-45)
