@@ -1,0 +1,690 @@
+// groupnorm.hip -- group norm with an activation over rows of channels (channels last), for the graphs of a batch (ragged segments of
+// rows, graph_ptr) and for dense samples of equal length (dgcnn_group_norm_fwd, dgcnn_group_norm_bwd).
+//
+//   per segment and group of D = C / G channels, n rows:   mu = mean x   var = mean (x - mu)^2   r = 1 / sqrt(var + eps)
+//   h = (x - mu) r     z = h w + b     y = act(z)
+//   q = dy act'(z)     db = sum q      dw = sum q h     a = mean(q w)    c = mean(q w h)     dx = r (q w - a - h c)
+//
+// Bound: HBM (forward x in, y out; backward x and dy in, dx out).  The tensor is cut into CHUNKS of R rows, R such that a workgroup holds a
+// chunk in registers (NV vectors a thread), and every row is read once into registers, whatever the segments' lengths:
+//   * a segment of at most R rows belongs to one workgroup: read once, statistics over the registers (mean first, then the squares
+//     of the differences: no cancellation), written once;
+//   * a longer segment is the business of the chunks it spans: each leaves its partial (mean, M2) per group -- slot = chunk + segment, unique
+//     because (chunk, segment) pairs form a staircase -- and a second launch combines the partials of the segment (a few KB, from L2) and
+//     reads its chunk once more (from the last-level cache when the tensor fits it).
+// Lengths are known on the device alone, so both run in ONE launch (workgroups 0..segments-1 and the chunks behind them), and the second launch
+// is left out when the host knows that no segment can be longer than R (few rows, or equal lengths).  Nothing is summed by atomics: every
+// sum has one order.
+// A thread keeps one column (VEC channels of one group) and every RY-th row; sums over a group go through one LDS slot a thread.
+// Statistics, partials and dw / db sums are fp32; y and dx are rounded once.
+#include "dg_half.h"
+
+#define GN_T 256             // threads of a workgroup, at least
+// ... and at most, which is also how many vectors a group may be wide: 1024 threads leave 128 registers each, which wide vectors' arithmetic
+// (w, b, the sums of dw and db) spills
+static constexpr int gn_most(int vec) { return vec >= 4 ? 512 : 1024; }
+#define GN_WROWS 1024        // workgroups that keep dw / db sums (rows of partial sums)
+
+struct DgGn {
+  const void *x, *dy, *w, *b;
+  void* out;                     // y or dx
+  const int64_t* ptr;            // null: B samples of `per` rows
+  float *mean, *rstd;            // [B][G]
+  float *part;                   // [chunks + B][G][2]
+  float *wpart;                  // [wrows][2][C]
+  int64_t N, per;
+  int B, C, G, D, DV, Gt, CVt, RY, R, P;      // D channels = DV vectors a group; Gt groups (CVt vectors) a workgroup; R = RY * NV rows a chunk; P lanes sum a group
+  int nseg;                      // workgroups that own whole segments
+  int nchunk, cgrid;             // chunks; workgroups that walk them (0: no segment is split)
+  int wdt, act, relaxed;         // type of w and b; activation; 1: a long segment is streamed by its workgroup (no second launch)
+  float eps;
+};
+
+// one vector's arithmetic at a time (one element's where it is an erf): interleaved by the scheduler they spill
+#define GN_FENCE() __builtin_amdgcn_sched_barrier(0)
+
+// ---- activation ------------------------------------------------------------------------------------------------------------------
+// v_exp_f32 and v_rcp_f32 are good to 1 ulp: exp(-z) carries |z| * 2^-24 * 1.44 of relative error, which the sigmoid's own decay outruns
+__device__ __forceinline__ float gn_sigmoid(float z) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.4426950408889634f * z)); }
+__device__ __forceinline__ float gn_tanh(float z) {
+  // the quotient form loses the value's own scale near 0; there the Taylor series (next term: 0.009 z^11, below 2^-24 of z for |z| < 0.3)
+  const float a = fabsf(z), u = z * z;
+  const float e = __builtin_amdgcn_exp2f(-2.8853900817779268f * a);
+  const float t = copysignf((1.f - e) * __builtin_amdgcn_rcpf(1.f + e), z);
+  const float s = z * (1.f + u * (-0.33333334f + u * (0.13333334f + u * (-0.053968254f + u * 0.021869488f))));
+  return a < 0.3f ? s : t;      // (NaN takes t)
+}
+template <int VEC> __device__ __forceinline__ void gn_act(int act, float* z) {
+  switch (act) {
+    case DGCNN_ACT_RELU:
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) z[i] = z[i] > 0.f ? z[i] : z[i] != z[i] ? z[i] : 0.f;
+      break;
+    case DGCNN_ACT_SILU:
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) z[i] = z[i] * gn_sigmoid(z[i]);
+      break;
+    case DGCNN_ACT_GELU:
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) { z[i] = 0.5f * z[i] * (1.f + erff(z[i] * 0.70710678f)); GN_FENCE(); }
+      break;
+    case DGCNN_ACT_TANH:
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) z[i] = gn_tanh(z[i]);
+      break;
+    default: break;
+  }
+}
+// z -> act'(z)
+template <int VEC> __device__ __forceinline__ void gn_slope(int act, float* z) {
+  switch (act) {
+    case DGCNN_ACT_RELU:
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) z[i] = z[i] > 0.f ? 1.f : z[i] != z[i] ? z[i] : 0.f;
+      break;
+    case DGCNN_ACT_SILU:
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) { const float s = gn_sigmoid(z[i]); z[i] = s * (1.f + z[i] * (1.f - s)); }
+      break;
+    case DGCNN_ACT_GELU:
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        z[i] = 0.5f * (1.f + erff(z[i] * 0.70710678f)) + z[i] * 0.3989422804f * __builtin_amdgcn_exp2f(-0.72134752f * z[i] * z[i]);
+        GN_FENCE();
+      }
+      break;
+    case DGCNN_ACT_TANH:
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) { const float t = gn_tanh(z[i]); z[i] = (1.f - t) * (1.f + t); }
+      break;
+    default:
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) z[i] = 1.f;
+  }
+}
+
+// ---- segments --------------------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ int64_t gn_uniform(int64_t v) {      // (the same in every lane: into scalar registers)
+  return (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)((uint64_t)v >> 32)) << 32) | (uint32_t)__builtin_amdgcn_readfirstlane((int)v));
+}
+// rows of segment s; whatever ptr holds, the range lies inside [0, N]
+__device__ __forceinline__ void gn_range(const DgGn& a, int s, int64_t& lo, int64_t& hi) {
+  if (a.ptr) {
+    lo = min(max(gn_uniform(a.ptr[s]), (int64_t)0), a.N);
+    hi = min(max(gn_uniform(a.ptr[s + 1]), lo), a.N);
+  } else {
+    lo = (int64_t)s * a.per;
+    hi = lo + a.per;
+  }
+}
+// the segment that row r lies in (-1: in front of the first; B: behind the last), found by the whole wave: 64 probes a step
+__device__ __forceinline__ int gn_find(const DgGn& a, int64_t r) {
+  if (!a.ptr) return (int)(r / a.per);
+  const int lane = threadIdx.x & 63;
+  int64_t lo = 0, hi = a.B + 1;
+  while (lo < hi) {
+    const int64_t step = (hi - lo + 63) >> 6, at = lo + lane * step;
+    const int n = __popcll(__ballot(at < hi && a.ptr[min(at, (int64_t)a.B)] <= r));
+    if (n == 0) break;
+    hi = min(hi, lo + (int64_t)n * step);
+    lo += (int64_t)(n - 1) * step + 1;
+  }
+  return (int)lo - 1;
+}
+
+// ---- sums over a group -----------------------------------------------------------------------------------------------------------
+struct GnLds { float red[2][1024]; float stat[2][1024]; };
+struct GnLane {
+  int t, r, c, g, slot;      // row and vector column inside the chunk, group inside the workgroup's, LDS slot (a group's slots are contiguous)
+  unsigned off;              // of the thread's vector in row block 0
+  bool on;                   // the thread owns a column (else r lies behind every row)
+};
+// every thread's u (and v) summed over its group -> L.stat[0/1][group].  Two barriers a sum; the first one of the next sum is what keeps this one's
+// results in place until everyone has read them.
+template <bool TWO> __device__ __forceinline__ void gn_sum(const DgGn& a, GnLds& L, const GnLane& me, int gn, float u, float v) {
+  if (me.on) { L.red[0][me.slot] = u; if (TWO) L.red[1][me.slot] = v; }
+  __syncthreads();
+  const int items = a.RY * a.DV, g = me.t / a.P, l = me.t & (a.P - 1);
+  float su = 0.f, sv = 0.f;
+  if (g < gn)
+    for (int j = l; j < items; j += a.P) { su += L.red[0][g * items + j]; if (TWO) sv += L.red[1][g * items + j]; }
+  for (int o = a.P >> 1; o; o >>= 1) { su += __shfl_xor(su, o); if (TWO) sv += __shfl_xor(sv, o); }
+  if (g < gn && l == 0) { L.stat[0][g] = su; if (TWO) L.stat[1][g] = sv; }
+  __syncthreads();
+}
+
+template <class D, int VEC> __device__ __forceinline__ void gn_zero_rows(const DgGn& a, const GnLane& me, int64_t lo, int64_t hi) {
+  for (int64_t at = lo; at < hi; at += a.RY)
+    if (me.r < hi - at) dg_store<D, VEC>(static_cast<typename D::S*>(a.out) + at * a.C + me.off, dg_zero<D, VEC>());
+}
+
+#define GN_SETUP()                                                                                                     \
+  __shared__ GnLds L;                                                                                                  \
+  const int g0 = blockIdx.y * a.Gt, gn = min(a.Gt, a.G - g0);                                                          \
+  GnLane me;                                                                                                           \
+  me.t = threadIdx.x; me.r = me.t / a.CVt; me.c = me.t - me.r * a.CVt; me.g = me.c / a.DV;                             \
+  me.on = me.r < a.RY && me.g < gn;                                                                                    \
+  me.slot = me.g * (a.RY * a.DV) + me.r * a.DV + (me.c - me.g * a.DV);                                                 \
+  const int ch = (g0 * a.DV + me.c) * VEC;      /* first channel of the thread */                                      \
+  me.off = (unsigned)me.r * a.C + ch;                                                                                  \
+  if (!me.on) me.r = 1 << 30;                                                                                          \
+  typedef typename D::S S;                                                                                             \
+  const S* const x = static_cast<const S*>(a.x);                                                                       \
+  S* const out = static_cast<S*>(a.out);                                                                               \
+  float w[VEC], b[VEC];                                                                                                \
+  _Pragma("unroll") for (int i = 0; i < VEC; ++i) {                                                                    \
+    w[i] = a.w && me.on ? dg_load_as(a.w, ch + i, a.wdt) : 1.f;                                                        \
+    b[i] = a.b && me.on ? dg_load_as(a.b, ch + i, a.wdt) : 0.f;                                                        \
+  }                                                                                                                    \
+  (void)x; (void)out; (void)b; (void)ch
+
+// Rows are addressed as (uniform base of the row block i RY) + (the thread's own 32-bit offset): a 64-bit address a row and thread would take
+// more registers than the rows.  `left` rows are there; a thread without a column has r beyond every `left`.
+template <class D, int VEC, int NV> __device__ __forceinline__ void gn_load(const DgGn& a, const GnLane& me, const typename D::S* p, int64_t at, int left, DgRaw<D, VEC>* v) {
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    v[i] = dg_zero<D, VEC>();
+    if (me.r < left - i * a.RY) v[i] = dg_load<D, VEC>(p + (at + (int64_t)i * a.RY) * a.C + me.off);
+  }
+}
+__device__ __forceinline__ int gn_left(const DgGn& a, int64_t at, int64_t hi) { return (int)min(hi - at, (int64_t)a.R); }
+
+template <class D, int VEC> __device__ __forceinline__ DgRaw<D, VEC> gn_apply(const DgGn& a, const DgRaw<D, VEC>& v, float mu, float rs, const float* w, const float* b) {
+  float z[VEC];
+  DgRaw<D, VEC> o;
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) z[e] = (v.get(e) - mu) * rs * w[e] + b[e];
+  gn_act<VEC>(a.act, z);
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) o.set(e, z[e]);
+  return o;
+}
+
+// What a workgroup of the first launch works on, one item after the other: segments q, q + 1, ... < end (whole, slot < 0), or the rows of long
+// segments inside the chunks k, k + cgrid, ...
+struct GnWork {
+  int64_t lo, hi;
+  int s, slot;
+  int next, end, k;
+  __device__ __forceinline__ GnWork(const DgGn& a) {
+    if ((int)blockIdx.x < a.nseg) {
+      next = (int)((int64_t)blockIdx.x * a.B / a.nseg); end = (int)((int64_t)(blockIdx.x + 1) * a.B / a.nseg) - 1; k = -1;
+    } else {
+      next = 0; end = -1; k = (int)blockIdx.x - a.nseg - a.cgrid;
+    }
+  }
+  // the next item with rows; false: done.  Uniform over the workgroup.  `empty(s)` is called for a segment without rows.
+  template <class Z> __device__ __forceinline__ bool fetch(const DgGn& a, Z empty) {
+    for (;;) {
+      if ((int)blockIdx.x < a.nseg) {
+        if (next > end) return false;
+        s = next++; slot = -1;
+        gn_range(a, s, lo, hi);
+        if (lo == hi) { empty(s); continue; }
+        if (hi - lo > a.R && !a.relaxed) continue;
+        return true;
+      }
+      if (next > end) {
+        k += a.cgrid;
+        if (k >= a.nchunk) return false;
+        const int64_t r0 = (int64_t)k * a.R, r1 = min(r0 + a.R, a.N);
+        next = max(gn_find(a, r0), 0); end = min(gn_find(a, r1 - 1), a.B - 1);
+        continue;
+      }
+      s = next; slot = k + s;
+      next = s < end ? end : end + 1;      // (a segment longer than a chunk is the chunk's first or its last)
+      gn_range(a, s, lo, hi);
+      if (hi - lo <= a.R) continue;
+      lo = max(lo, (int64_t)k * a.R); hi = min(hi, (int64_t)(k + 1) * a.R);
+      if (lo < hi) return true;
+    }
+  }
+};
+// without a second launch, the rows outside every segment are cleared by the workgroups of the first and the last one
+template <class D, int VEC> __device__ __forceinline__ void gn_clear(const DgGn& a, const GnLane& me) {
+  if (a.cgrid) return;
+  int64_t lo, hi;
+  if (blockIdx.x == 0) { gn_range(a, 0, lo, hi); gn_zero_rows<D, VEC>(a, me, 0, lo); }
+  if ((int)blockIdx.x == a.nseg - 1) { gn_range(a, a.B - 1, lo, hi); gn_zero_rows<D, VEC>(a, me, hi, a.N); }
+}
+
+// forward: whole segments, and the partial moments of the chunks of long ones.  More than R rows (a few long segments, no second launch) pass
+// through the registers piece by piece, read again for each of the three passes.
+template <class D, int VEC, int NV>
+__global__ void __launch_bounds__(gn_most(VEC))
+k_gn_fwd(const DgGn a) {
+  GN_SETUP();
+  DgRaw<D, VEC> v[NV];
+  gn_clear<D, VEC>(a, me);
+  GnWork it(a);
+  while (it.fetch(a, [&](int s) {
+    if (me.t < gn) { a.mean[(int64_t)s * a.G + g0 + me.t] = 0.f; a.rstd[(int64_t)s * a.G + g0 + me.t] = 0.f; }
+  })) {
+    const bool again = it.hi - it.lo > a.R;
+    const float n = (float)(it.hi - it.lo) * (float)a.D;
+    float sum = 0.f, sq = 0.f;
+    for (int64_t at = it.lo; at < it.hi; at += a.R) {
+      const int left = gn_left(a, at, it.hi);
+      gn_load<D, VEC, NV>(a, me, x, at, left, v);
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) sum += v[i].get(e);
+    }
+    gn_sum<false>(a, L, me, gn, sum, 0.f);
+    dg_hide<D, VEC, NV>(v);
+    const float mu = me.on ? L.stat[0][me.g] / n : 0.f;      // (divided: a constant segment's mean is the constant, its squares' sum 0)
+    for (int64_t at = it.lo; at < it.hi; at += a.R) {
+      const int left = gn_left(a, at, it.hi);
+      if (again) gn_load<D, VEC, NV>(a, me, x, at, left, v);
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        if (me.r < left - i * a.RY) {
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) { const float d = v[i].get(e) - mu; sq += d * d; }
+        }
+    }
+    gn_sum<false>(a, L, me, gn, sq, 0.f);
+    dg_hide<D, VEC, NV>(v);
+    const bool first = me.r == 0 && me.c == me.g * a.DV;      // one thread of each group
+    if (it.slot >= 0) {
+      if (first) {
+        float* const p = a.part + ((int64_t)it.slot * a.G + g0 + me.g) * 2;
+        p[0] = mu; p[1] = L.stat[0][me.g];
+      }
+      continue;
+    }
+    const float rs = me.on ? 1.f / sqrtf(L.stat[0][me.g] / n + a.eps) : 0.f;
+    if (first) { a.mean[(int64_t)it.s * a.G + g0 + me.g] = mu; a.rstd[(int64_t)it.s * a.G + g0 + me.g] = rs; }
+    for (int64_t at = it.lo; at < it.hi; at += a.R) {
+      const int left = gn_left(a, at, it.hi);
+      if (again) gn_load<D, VEC, NV>(a, me, x, at, left, v);
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        if (me.r < left - i * a.RY) dg_store<D, VEC>(out + (at + (int64_t)i * a.RY) * a.C + me.off, gn_apply<D, VEC>(a, v[i], mu, rs, w, b));
+        GN_FENCE();
+      }
+    }
+  }
+}
+
+// the chunks of long segments: partial moments -> mean, rstd -> y; rows outside every segment -> 0
+template <class D, int VEC, int NV>
+__global__ void __launch_bounds__(gn_most(VEC))
+k_gn_fwd_long(const DgGn a) {
+  GN_SETUP();
+  for (int k = blockIdx.x; k < a.nchunk; k += gridDim.x) {
+    const int64_t r0 = (int64_t)k * a.R, r1 = min(r0 + a.R, a.N);
+    const int f0 = gn_find(a, r0), f1 = gn_find(a, r1 - 1);
+    if (f0 < 0 || f1 >= a.B) {
+      int64_t lo, hi, u;
+      gn_range(a, 0, lo, u);
+      gn_range(a, a.B - 1, u, hi);
+      if (f0 < 0) gn_zero_rows<D, VEC>(a, me, r0, min(lo, r1));
+      if (f1 >= a.B) gn_zero_rows<D, VEC>(a, me, max(hi, r0), r1);
+    }
+    const int s0 = max(f0, 0), s1 = min(f1, a.B - 1);
+    for (int s = s0; s <= s1; s = s < s1 ? s1 : s1 + 1) {
+      int64_t lo, hi;
+      gn_range(a, s, lo, hi);
+      if (hi - lo <= a.R) continue;
+      const int64_t a0 = max(lo, r0), a1 = min(hi, r1);
+      if (a0 >= a1) continue;
+      const int left = (int)(a1 - a0);
+      DgRaw<D, VEC> v[NV];
+      gn_load<D, VEC, NV>(a, me, x, a0, left, v);      // (in flight while the partials are combined)
+      // mean = sum n_i mean_i / n;   M2 = sum M2_i + n_i (mean_i - mean)^2
+      const int k0 = (int)(lo / a.R), k1 = (int)((hi - 1) / a.R), g = me.t / a.P, l = me.t & (a.P - 1);
+      const float* const p = a.part + ((int64_t)(k0 + s) * a.G + g0 + g) * 2;
+      const float n = (float)(hi - lo);
+      float m = 0.f, q = 0.f;
+      if (g < gn)
+        for (int i = l; i <= k1 - k0; i += a.P)
+          m += p[(int64_t)i * a.G * 2] * (float)(min((int64_t)(k0 + i + 1) * a.R, hi) - max((int64_t)(k0 + i) * a.R, lo));
+      for (int o = a.P >> 1; o; o >>= 1) m += __shfl_xor(m, o);
+      m /= n;
+      if (g < gn)
+        for (int i = l; i <= k1 - k0; i += a.P) {
+          const float d = p[(int64_t)i * a.G * 2] - m;
+          q += p[(int64_t)i * a.G * 2 + 1] + (float)(min((int64_t)(k0 + i + 1) * a.R, hi) - max((int64_t)(k0 + i) * a.R, lo)) * (float)a.D * d * d;
+        }
+      for (int o = a.P >> 1; o; o >>= 1) q += __shfl_xor(q, o);
+      if (g < gn && l == 0) {
+        const float rs = 1.f / sqrtf(q / n / (float)a.D + a.eps);
+        L.stat[0][g] = m; L.stat[1][g] = rs;
+        if (k == k0) { a.mean[(int64_t)s * a.G + g0 + g] = m; a.rstd[(int64_t)s * a.G + g0 + g] = rs; }
+      }
+      __syncthreads();
+      const float mu = me.on ? L.stat[0][me.g] : 0.f, rs = me.on ? L.stat[1][me.g] : 0.f;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        if (me.r < left - i * a.RY) dg_store<D, VEC>(out + (a0 + (int64_t)i * a.RY) * a.C + me.off, gn_apply<D, VEC>(a, v[i], mu, rs, w, b));
+        GN_FENCE();
+      }
+      __syncthreads();
+    }
+  }
+}
+
+// ---- backward --------------------------------------------------------------------------------------------------------------------
+// h and q of one vector
+template <class D, int VEC> __device__ __forceinline__ void gn_hq(const DgGn& a, const DgRaw<D, VEC>& x, const DgRaw<D, VEC>& dy, float mu, float rs, const float* w, const float* b, float* h, float* q) {
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) { h[e] = (x.get(e) - mu) * rs; q[e] = h[e] * w[e] + b[e]; }
+  gn_slope<VEC>(a.act, q);
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) q[e] *= dy.get(e);
+}
+template <class D, int VEC> __device__ __forceinline__ DgRaw<D, VEC> gn_dx(const DgGn& a, const DgRaw<D, VEC>& x, const DgRaw<D, VEC>& dy, float mu, float rs, const float* w, const float* b, float am, float cm) {
+  float h[VEC], q[VEC];
+  gn_hq<D, VEC>(a, x, dy, mu, rs, w, b, h, q);
+  DgRaw<D, VEC> o;
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) o.set(e, rs * (q[e] * w[e] - am - h[e] * cm));
+  return o;
+}
+// one vector into the thread's sums
+template <class D, int VEC> __device__ __forceinline__ void gn_add(const DgGn& a, const DgRaw<D, VEC>& x, const DgRaw<D, VEC>& dy, float mu, float rs, const float* w, const float* b, float* dw, float* db, float& s1, float& s2) {
+  float h[VEC], q[VEC];
+  gn_hq<D, VEC>(a, x, dy, mu, rs, w, b, h, q);
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) {
+    db[e] += q[e];
+    dw[e] += q[e] * h[e];
+    const float qw = q[e] * w[e];
+    s1 += qw; s2 += qw * h[e];
+  }
+}
+// the workgroup's dw, db sums -> its row of wpart
+template <int VEC> __device__ __forceinline__ void gn_put_w(const DgGn& a, GnLds& L, const GnLane& me, int gn, int ch, const float* dw, const float* db) {
+  float* const row = a.wpart + (int64_t)blockIdx.x * 2 * a.C;
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) {
+    __syncthreads();
+    if (me.on) { L.red[0][me.t] = dw[e]; L.red[1][me.t] = db[e]; }
+    __syncthreads();
+    if (me.on && me.r == 0) {
+      float u = 0.f, v = 0.f;
+      for (int r = 0; r < a.RY; ++r) { u += L.red[0][r * a.CVt + me.t]; v += L.red[1][r * a.CVt + me.t]; }
+      row[ch + e] = u; row[a.C + ch + e] = v;
+    }
+  }
+}
+
+// backward: whole segments (each workgroup walks a contiguous share of them), and the partial sums of the chunks of long ones
+template <class D, int VEC, int NV>
+__global__ void __launch_bounds__(gn_most(VEC))
+k_gn_bwd(const DgGn a) {
+  GN_SETUP();
+  const S* const dy = static_cast<const S*>(a.dy);
+  DgRaw<D, VEC> v[NV], d[NV];
+  float dw[VEC], db[VEC];
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) dw[e] = db[e] = 0.f;
+  gn_clear<D, VEC>(a, me);
+  GnWork it(a);
+  while (it.fetch(a, [](int) {})) {
+    const bool again = it.hi - it.lo > a.R;
+    const float inv_n = 1.f / ((float)(it.hi - it.lo) * (float)a.D);
+    float mu = me.on ? a.mean[(int64_t)it.s * a.G + g0 + me.g] : 0.f;
+    const float rs = me.on ? a.rstd[(int64_t)it.s * a.G + g0 + me.g] : 0.f;
+    float s1 = 0.f, s2 = 0.f;
+    for (int64_t at = it.lo; at < it.hi; at += a.R) {
+      const int left = gn_left(a, at, it.hi);
+      gn_load<D, VEC, NV>(a, me, x, at, left, v);
+      gn_load<D, VEC, NV>(a, me, dy, at, left, d);
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        { if (me.r < left - i * a.RY) gn_add<D, VEC>(a, v[i], d[i], mu, rs, w, b, dw, db, s1, s2); GN_FENCE(); }
+    }
+    gn_sum<true>(a, L, me, gn, s1, s2);
+    if (it.slot >= 0) {
+      if (me.t < gn) {
+        float* const p = a.part + ((int64_t)it.slot * a.G + g0 + me.t) * 2;
+        p[0] = L.stat[0][me.t]; p[1] = L.stat[1][me.t];
+      }
+      continue;
+    }
+    dg_hide<D, VEC, NV>(v);      // (h and q are computed again: held over the sum they take twice the registers of x and dy)
+    dg_hide<D, VEC, NV>(d);
+    DG_OPAQUE_V(mu);
+    const float am = me.on ? L.stat[0][me.g] * inv_n : 0.f, cm = me.on ? L.stat[1][me.g] * inv_n : 0.f;
+    for (int64_t at = it.lo; at < it.hi; at += a.R) {
+      const int left = gn_left(a, at, it.hi);
+      if (again) { gn_load<D, VEC, NV>(a, me, x, at, left, v); gn_load<D, VEC, NV>(a, me, dy, at, left, d); }
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        if (me.r < left - i * a.RY) dg_store<D, VEC>(out + (at + (int64_t)i * a.RY) * a.C + me.off, gn_dx<D, VEC>(a, v[i], d[i], mu, rs, w, b, am, cm));
+        GN_FENCE();
+      }
+    }
+  }
+  if (a.wpart) gn_put_w<VEC>(a, L, me, gn, ch, dw, db);
+}
+
+template <class D, int VEC, int NV>
+__global__ void __launch_bounds__(gn_most(VEC))
+k_gn_bwd_long(const DgGn a) {
+  GN_SETUP();
+  const S* const dy = static_cast<const S*>(a.dy);
+  for (int k = blockIdx.x; k < a.nchunk; k += gridDim.x) {
+    const int64_t r0 = (int64_t)k * a.R, r1 = min(r0 + a.R, a.N);
+    const int f0 = gn_find(a, r0), f1 = gn_find(a, r1 - 1);
+    if (f0 < 0 || f1 >= a.B) {
+      int64_t lo, hi, u;
+      gn_range(a, 0, lo, u);
+      gn_range(a, a.B - 1, u, hi);
+      if (f0 < 0) gn_zero_rows<D, VEC>(a, me, r0, min(lo, r1));
+      if (f1 >= a.B) gn_zero_rows<D, VEC>(a, me, max(hi, r0), r1);
+    }
+    const int s0 = max(f0, 0), s1 = min(f1, a.B - 1);
+    for (int s = s0; s <= s1; s = s < s1 ? s1 : s1 + 1) {
+      int64_t lo, hi;
+      gn_range(a, s, lo, hi);
+      if (hi - lo <= a.R) continue;
+      const int64_t a0 = max(lo, r0), a1 = min(hi, r1);
+      if (a0 >= a1) continue;
+      const int left = (int)(a1 - a0);
+      DgRaw<D, VEC> v[NV], d[NV];
+      gn_load<D, VEC, NV>(a, me, x, a0, left, v);
+      gn_load<D, VEC, NV>(a, me, dy, a0, left, d);
+      const int k0 = (int)(lo / a.R), k1 = (int)((hi - 1) / a.R), g = me.t / a.P, l = me.t & (a.P - 1);
+      const float* const p = a.part + ((int64_t)(k0 + s) * a.G + g0 + g) * 2;
+      float u1 = 0.f, u2 = 0.f;
+      if (g < gn)
+        for (int i = l; i <= k1 - k0; i += a.P) { u1 += p[(int64_t)i * a.G * 2]; u2 += p[(int64_t)i * a.G * 2 + 1]; }
+      for (int o = a.P >> 1; o; o >>= 1) { u1 += __shfl_xor(u1, o); u2 += __shfl_xor(u2, o); }
+      if (g < gn && l == 0) {
+        const float inv_n = 1.f / ((float)(hi - lo) * (float)a.D);
+        L.stat[0][g] = u1 * inv_n; L.stat[1][g] = u2 * inv_n;
+      }
+      __syncthreads();
+      const float am = me.on ? L.stat[0][me.g] : 0.f, cm = me.on ? L.stat[1][me.g] : 0.f;
+      const float mu = me.on ? a.mean[(int64_t)s * a.G + g0 + me.g] : 0.f, rs = me.on ? a.rstd[(int64_t)s * a.G + g0 + me.g] : 0.f;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        if (me.r < left - i * a.RY) dg_store<D, VEC>(out + (a0 + (int64_t)i * a.RY) * a.C + me.off, gn_dx<D, VEC>(a, v[i], d[i], mu, rs, w, b, am, cm));
+        GN_FENCE();
+      }
+      __syncthreads();
+    }
+  }
+}
+
+// dw, db: the workgroups' rows summed column by column, in a fixed order: 16 columns x 64 row lanes
+__global__ void __launch_bounds__(1024)
+k_gn_wsum(const float* __restrict__ part, int rows, int C, void* dw, void* db, int dt) {
+  __shared__ float red[64][17];
+  const int col = blockIdx.x * 16 + (threadIdx.x & 15), lane = threadIdx.x >> 4;
+  float s = 0.f;
+  if (col < 2 * C)
+    for (int r = lane; r < rows; r += 64) s += part[(int64_t)r * 2 * C + col];
+  red[lane][threadIdx.x & 15] = s;
+  __syncthreads();
+  for (int o = 32; o; o >>= 1) {
+    if (lane < o) red[lane][threadIdx.x & 15] += red[lane + o][threadIdx.x & 15];
+    __syncthreads();
+  }
+  if (lane == 0 && col < 2 * C) {
+    void* const out = col < C ? dw : db;
+    if (out) dg_store_as(out, col < C ? col : col - C, dt, red[0][threadIdx.x & 15]);
+  }
+}
+
+// ---- host ------------------------------------------------------------------------------------------------------------------------
+// vectors a thread holds: 8 of x, or 4 of x and dy (32 registers); twice as many where a vector is one register or half of one
+static constexpr int gn_nv(int vec_bytes, bool bwd) { return (bwd ? 4 : 8) * (vec_bytes <= 4 ? 2 : 1); }
+
+// everything that follows from the shape; false: the shape is outside what this build handles
+static bool gn_plan(DgGn* a, int dtype, int vec_cap, bool bwd, int* vec, int* threads, int* tiles) {
+  const int full = dtype == DGCNN_F32 ? 4 : 8;
+  int v = full < vec_cap ? full : vec_cap;
+  while (a->D % v) v >>= 1;
+  a->DV = a->D / v;
+  const int most = gn_most(v);
+  if (a->DV > most) return false;
+  const int nv = gn_nv(v * dg_dtype_size(dtype), bwd), cols = a->DV * a->G;
+  int t = GN_T;
+  while (t < most && (a->DV > t || cols > t)) t *= 2;      // one column tile if the threads suffice
+  a->Gt = cols <= t ? a->G : t / a->DV;
+  a->CVt = a->Gt * a->DV;
+  // a wider workgroup where that lets it hold segments of up to twice the average length (they differ); where none could, many small chunks
+  const int64_t want = a->B ? 2 * ((a->N + a->B - 1) / a->B) : 0;
+  if ((int64_t)(most / a->CVt) * nv >= want)
+    while (t < most && (int64_t)(t / a->CVt) * nv < want) t *= 2;
+  a->RY = t / a->CVt;
+  a->R = a->RY * nv;
+  a->P = 64;
+  while (a->P > 1 && a->P * a->Gt > t) a->P >>= 1;
+  *vec = v; *threads = t; *tiles = (a->G + a->Gt - 1) / a->Gt;
+  return true;
+}
+// which workgroups run: see the head of the file
+static void gn_grid(DgGn* a, int es, bool bwd) {
+  const bool one_long = a->ptr ? a->N > a->R : a->per > a->R;      // can any segment be longer than a chunk?
+  const bool all_long = !a->ptr && a->per > a->R;                  // are all?
+  // A long segment is worth a second launch (2 us) from 256 KB on: one workgroup streams ~100 bytes a nanosecond.
+  a->relaxed = one_long && a->N * a->C * es <= 256 * 1024;
+  const bool split = one_long && !a->relaxed;
+  a->nseg = all_long && split ? 0 : bwd && a->B > GN_WROWS ? GN_WROWS : a->B;
+  a->nchunk = split ? (int)((a->N + a->R - 1) / a->R) : 0;
+  a->cgrid = a->nchunk < GN_WROWS ? a->nchunk : GN_WROWS;
+}
+static bool gn_shape(DgGn* a, int64_t rows, int C, int groups, int segments) {
+  if (rows < 0 || C < 1 || groups < 1 || C % groups || segments < 0) return false;
+  a->N = rows; a->B = segments; a->C = C; a->G = groups; a->D = C / groups;
+  return true;
+}
+static int64_t gn_part_bytes(const DgGn& a) { return dg_align(((int64_t)a.nchunk + a.B) * a.G * 2 * 4, 256); }
+
+// the plan of a call; alignment of the tensors (a multiple of the vector's bytes) is known at the call only, so the workspace is for the worst
+extern "C" int64_t dgcnn_group_norm_workspace_bytes(int64_t rows, int C, int groups, int segments, int dense, int dtype, int backward) {
+  DgGn a = {};
+  if (!gn_shape(&a, rows, C, groups, segments) || !dg_dtype_ok(dtype)) return DGCNN_EINVAL;
+  if (segments == 0 || rows == 0) return 256;
+  if (rows > ((int64_t)1 << 40) / C) return DGCNN_EUNSUPPORTED;
+  static const int64_t dummy[2] = {0, 0};
+  int64_t most = 256;
+  for (int cap = 8; cap >= 1; cap >>= 1) {
+    int v, t, n;
+    a.ptr = dense ? nullptr : dummy;
+    a.per = dense ? rows / segments : 0;
+    if (!gn_plan(&a, dtype, cap, backward != 0, &v, &t, &n)) continue;
+    gn_grid(&a, dg_dtype_size(dtype), backward != 0);
+    const int64_t b = (a.nchunk ? gn_part_bytes(a) : 0) + (backward ? dg_align(((int64_t)a.nseg + a.cgrid) * 2 * C * 4, 256) : 0);
+    if (b > most) most = b;
+  }
+  return most;
+}
+
+typedef void (*gn_kernel)(const DgGn);
+template <class D, int VEC> static gn_kernel gn_pick(int which) {
+  constexpr int F = gn_nv(VEC * sizeof(typename D::S), false), W = gn_nv(VEC * sizeof(typename D::S), true);
+  switch (which) {
+    case 0: return (gn_kernel)k_gn_fwd<D, VEC, F>;
+    case 1: return (gn_kernel)k_gn_fwd_long<D, VEC, F>;
+    case 2: return (gn_kernel)k_gn_bwd<D, VEC, W>;
+    default: return (gn_kernel)k_gn_bwd_long<D, VEC, W>;
+  }
+}
+template <class D> static gn_kernel gn_pick_vec(int vec, int which) {
+  if constexpr (D::FULL == 8) { if (vec == 8) return gn_pick<D, 8>(which); }
+  return vec == 4 ? gn_pick<D, 4>(which) : vec == 2 ? gn_pick<D, 2>(which) : gn_pick<D, 1>(which);
+}
+static gn_kernel gn_pick_dtype(int dtype, int vec, int which) {
+  return dtype == DGCNN_F32 ? gn_pick_vec<DgF32>(vec, which) : dtype == DGCNN_BF16 ? gn_pick_vec<DgBF16>(vec, which) : gn_pick_vec<DgF16>(vec, which);
+}
+// largest vector (in elements) that every address in `low` and the row length admit
+static int gn_vec_cap(uintptr_t low, int C, int es) {
+  int v = 16 / es;
+  while (v > 1 && ((low & (uintptr_t)(v * es - 1)) || C % v)) v >>= 1;
+  return v;
+}
+static int gn_check(const dgcnn_group_norm_args* p, DgGn* a) {
+  if (!p || !gn_shape(a, p->rows, p->channels, p->groups, p->segments)) return DGCNN_EINVAL;
+  if (!dg_dtype_ok(p->dtype) || ((p->weight || p->bias) && !dg_dtype_ok(p->weight_dtype))) return DGCNN_EINVAL;
+  if (p->act < DGCNN_ACT_NONE || p->act > DGCNN_ACT_TANH || !(p->eps >= 0.f)) return DGCNN_EINVAL;
+  if (p->rows > 0 && p->segments > 0 && (!p->x || !p->mean || !p->rstd)) return DGCNN_EINVAL;
+  if (!p->ptr && p->segments > 0 && p->rows % p->segments) return DGCNN_EINVAL;
+  if (!p->ptr && p->segments == 0 && p->rows > 0) return DGCNN_EINVAL;
+  if (p->rows > ((int64_t)1 << 40) / p->channels) return DGCNN_EUNSUPPORTED;
+  a->x = p->x; a->w = p->weight; a->b = p->bias; a->ptr = p->ptr; a->mean = p->mean; a->rstd = p->rstd;
+  a->per = !p->ptr && p->segments ? p->rows / p->segments : 0;
+  a->wdt = p->weight_dtype; a->act = p->act; a->eps = p->eps;
+  return DGCNN_OK;
+}
+
+extern "C" int dgcnn_group_norm_fwd(const dgcnn_group_norm_args* p, void* y, void* ws, dgcnn_stream_t stream) {
+  DgGn a = {};
+  const int rc = gn_check(p, &a);
+  if (rc != DGCNN_OK) return rc;
+  if (p->rows == 0 || p->segments == 0) return DGCNN_OK;      // (no segment: nothing is written)
+  if (!y || !ws) return DGCNN_EINVAL;
+  a.out = y;
+  int vec, threads, tiles;
+  const int cap = gn_vec_cap(reinterpret_cast<uintptr_t>(p->x) | reinterpret_cast<uintptr_t>(y), a.C, dg_dtype_size(p->dtype));
+  if (!gn_plan(&a, p->dtype, cap, false, &vec, &threads, &tiles)) return DGCNN_EUNSUPPORTED;
+  gn_grid(&a, dg_dtype_size(p->dtype), false);
+  a.part = static_cast<float*>(ws);
+  hipLaunchKernelGGL(gn_pick_dtype(p->dtype, vec, 0), dim3(a.nseg + a.cgrid, tiles), dim3(threads), 0, (hipStream_t)stream, a);
+  DG_CHECK_LAUNCH();
+  if (a.cgrid) {
+    hipLaunchKernelGGL(gn_pick_dtype(p->dtype, vec, 1), dim3(a.nchunk, tiles), dim3(threads), 0, (hipStream_t)stream, a);
+    DG_CHECK_LAUNCH();
+  }
+  return DGCNN_OK;
+}
+
+extern "C" int dgcnn_group_norm_bwd(const dgcnn_group_norm_args* p, const void* dy, void* dx, void* dweight, void* dbias, void* ws, dgcnn_stream_t stream) {
+  DgGn a = {};
+  const int rc = gn_check(p, &a);
+  if (rc != DGCNN_OK) return rc;
+  if ((dweight || dbias) && !dg_dtype_ok(p->weight_dtype)) return DGCNN_EINVAL;
+  const bool none = p->rows == 0 || p->segments == 0;
+  if (!none && (!dy || !dx || !ws)) return DGCNN_EINVAL;
+  if (none) {      // (empty sums; dx has no row that lies in a segment)
+    if (dweight || dbias) {
+      hipLaunchKernelGGL(k_gn_wsum, dim3(dg_cdiv(2 * a.C, 16)), dim3(1024), 0, (hipStream_t)stream, (const float*)nullptr, 0, a.C, dweight, dbias, p->weight_dtype);
+      DG_CHECK_LAUNCH();
+    }
+    return DGCNN_OK;
+  }
+  a.dy = dy; a.out = dx;
+  int vec, threads, tiles;
+  const int cap = gn_vec_cap(reinterpret_cast<uintptr_t>(p->x) | reinterpret_cast<uintptr_t>(dy) | reinterpret_cast<uintptr_t>(dx), a.C, dg_dtype_size(p->dtype));
+  if (!gn_plan(&a, p->dtype, cap, true, &vec, &threads, &tiles)) return DGCNN_EUNSUPPORTED;
+  gn_grid(&a, dg_dtype_size(p->dtype), true);
+  a.part = static_cast<float*>(ws);
+  if (dweight || dbias) a.wpart = reinterpret_cast<float*>(static_cast<char*>(ws) + (a.nchunk ? gn_part_bytes(a) : 0));
+  hipLaunchKernelGGL(gn_pick_dtype(p->dtype, vec, 2), dim3(a.nseg + a.cgrid, tiles), dim3(threads), 0, (hipStream_t)stream, a);
+  DG_CHECK_LAUNCH();
+  if (a.cgrid) {
+    hipLaunchKernelGGL(gn_pick_dtype(p->dtype, vec, 3), dim3(a.nchunk, tiles), dim3(threads), 0, (hipStream_t)stream, a);
+    DG_CHECK_LAUNCH();
+  }
+  if (a.wpart) {
+    hipLaunchKernelGGL(k_gn_wsum, dim3(dg_cdiv(2 * a.C, 16)), dim3(1024), 0, (hipStream_t)stream, (const float*)a.wpart, a.nseg + a.cgrid, a.C, dweight, dbias, p->weight_dtype);
+    DG_CHECK_LAUNCH();
+  }
+  return DGCNN_OK;
+}
