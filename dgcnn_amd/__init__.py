@@ -6,7 +6,8 @@ Public surface (mirrors what the reference exposes for this path):
   Trainer          -- the per-batch step of /root/reference/train.py:27-66 on fused kernels
   optim.Adam       -- torch.optim.Adam drop-in that updates the flat parameter buffer with one kernel (train.py:11,99)
   optim.AdamW      -- AdamW over any list of GPU tensors in one launch, moments in 32 or 8 bits (optim.adamw_step: over plain lists)
-  layers           -- differentiable operators and modules over a batch's rows: group norm with an activation
+  layers           -- differentiable operators and modules over a batch's rows: products grouped by type, group norm with an
+                      activation
   device_data      -- DeviceDataset / DeviceLoader: dataset resident in HBM, batches assembled on the device
   tudataset        -- TU-format reader + Indegree + fold files + GraphLoader (train.py:81-109, utils.py:18-33)
   cli              -- the 10-fold driver (train.py:69-148), also reachable as ``python train.py``

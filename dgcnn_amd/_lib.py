@@ -85,6 +85,12 @@ class GroupNormArgs(ctypes.Structure):
                 ("mean", c_void_p), ("rstd", c_void_p)]
 
 
+class GroupedLinearArgs(ctypes.Structure):
+    """``dgcnn_grouped_linear_args`` of include/dgcnn_hip.h"""
+    _fields_ = [("rows", c_int64), ("ldx", c_int64), ("in_features", ctypes.c_int32), ("out_features", ctypes.c_int32),
+                ("groups", ctypes.c_int32), ("dtype", ctypes.c_int32), ("x", c_void_p), ("weight", c_void_p), ("bias", c_void_p), ("ptr", c_void_p)]
+
+
 # name -> (restype, argtypes); must list every symbol include/dgcnn_hip.h declares
 SIGNATURES = {
     "dgcnn_model_eval_step": (c_int, [ctypes.POINTER(StepArgs), c_void_p]),
@@ -125,6 +131,9 @@ SIGNATURES = {
     "dgcnn_adam_step": (c_int, [c_void_p] * 4 + [c_int64, c_int64, c_float, c_float, c_float, c_float, c_int,
                                 c_void_p]),
     "dgcnn_adamw_step": (c_int, [ctypes.POINTER(AdamwArgs), c_void_p]),
+    "dgcnn_grouped_linear_workspace_bytes": (c_int64, [c_int64] + [c_int] * 4),
+    "dgcnn_grouped_linear_fwd": (c_int, [ctypes.POINTER(GroupedLinearArgs)] + [c_void_p] * 2),
+    "dgcnn_grouped_linear_bwd": (c_int, [ctypes.POINTER(GroupedLinearArgs)] + [c_void_p] * 6),
     "dgcnn_group_norm_workspace_bytes": (c_int64, [c_int64] + [c_int] * 6),
     "dgcnn_group_norm_fwd": (c_int, [ctypes.POINTER(GroupNormArgs)] + [c_void_p] * 3),
     "dgcnn_group_norm_bwd": (c_int, [ctypes.POINTER(GroupNormArgs)] + [c_void_p] * 6),

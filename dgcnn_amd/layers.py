@@ -1,5 +1,6 @@
 """Layer operators for networks around the graph convolutions: differentiable functions and modules over the node rows of a batch.
 
+* :func:`grouped_linear` / :class:`GroupedLinear` -- a linear map for each type (relation, expert) of the rows, sorted by type.
 * :func:`group_norm` / :class:`GroupNorm` -- group norm with an activation, channels last, over every graph of a batch (``ptr``) or over dense
   samples ``[B, ..., C]``.
 
@@ -61,6 +62,89 @@ def graph_ptr(data) -> torch.Tensor:
     if n is None:
         n = int(batch[-1].item()) + 1 if batch.numel() else 0
     return torch.searchsorted(batch.contiguous(), torch.arange(n + 1, device=batch.device, dtype=batch.dtype))
+
+
+# ---- products grouped by type ----------------------------------------------------------------------------------------------------------
+class _GroupedLinear(torch.autograd.Function):
+    @staticmethod
+    def _args(x, weight, bias, ptr):
+        a = _lib.GroupedLinearArgs()
+        a.rows, a.in_features = x.shape
+        a.groups, a.out_features = weight.shape[:2]
+        a.ldx, a.dtype = max(x.stride(0), a.in_features), _DTYPES[x.dtype]
+        a.x, a.weight, a.ptr = x.data_ptr(), weight.data_ptr(), ptr.data_ptr()
+        a.bias = None if bias is None else bias.data_ptr()
+        return a
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, ptr):
+        if x.stride(1) != 1 or (x.shape[0] > 1 and x.stride(0) < x.shape[1]):
+            x = x.contiguous()
+        weight = weight.contiguous()
+        bias = None if bias is None else bias.contiguous()
+        a = _GroupedLinear._args(x, weight, bias, ptr)
+        y = torch.empty(a.rows, a.out_features, dtype=x.dtype, device=x.device)
+        with _on(x.device):
+            _lib.check(_lib.lib().dgcnn_grouped_linear_fwd(ctypes.byref(a), y.data_ptr(), _stream(x.device)), "dgcnn_grouped_linear_fwd")
+        ctx.save_for_backward(x, weight, bias, ptr)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, weight, bias, ptr = ctx.saved_tensors
+        a = _GroupedLinear._args(x, weight, bias, ptr)
+        dy = dy.contiguous()
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        dx = torch.empty(a.rows, a.in_features, dtype=x.dtype, device=x.device) if need_x else None
+        dw = torch.empty_like(weight) if need_w or need_b else None
+        db = torch.empty_like(bias) if need_b else None
+        L, ws = _lib.lib(), None
+        if dw is not None:
+            ws = torch.empty(_lib.checked_bytes(L.dgcnn_grouped_linear_workspace_bytes(a.rows, a.in_features, a.out_features, a.groups, a.dtype),
+                                                "dgcnn_grouped_linear_workspace_bytes"), dtype=torch.uint8, device=x.device)
+        at = lambda t: None if t is None else t.data_ptr()      # noqa: E731
+        with _on(x.device):
+            _lib.check(L.dgcnn_grouped_linear_bwd(ctypes.byref(a), dy.data_ptr(), at(dx), at(dw), at(db), at(ws), _stream(x.device)), "dgcnn_grouped_linear_bwd")
+        return dx, dw if need_w else None, db, None
+
+
+def grouped_linear(x: torch.Tensor, weight: torch.Tensor, ptr: torch.Tensor, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``y[i] = weight[e] @ x[i] + bias[e]`` for the rows ``ptr[e] <= i < ptr[e + 1]`` of every group ``e``: ``x`` [N, in] sorted by group, ``weight``
+    [groups, out, in] (as ``nn.Linear``'s), ``bias`` [groups, out], ``ptr`` [groups + 1] (ascending, on the device; never read by the host).
+
+    Groups may be empty; rows outside every group give 0 and get gradient 0.  Everything of one type; sums in fp32, results rounded once.  The rows
+    of ``x`` may be strided.  Differentiable once in ``x``, ``weight`` and ``bias``."""
+    _refuse(not x.is_cuda, "dgcnn_amd.layers runs only on an AMD GPU through libdgcnn_hip.so; got a CPU tensor (there is deliberately no CPU fallback)")
+    _refuse(x.dim() != 2 or weight.dim() != 3 or x.shape[1] != weight.shape[2] or min(weight.shape[1:]) < 1,
+            f"x must be [N, in] and weight [groups, out, in], got {tuple(x.shape)} and {tuple(weight.shape)}")
+    _dtype(x, "x")
+    _refuse(weight.dtype != x.dtype or weight.device != x.device, f"weight must be {x.dtype} on {x.device}, got {weight.dtype} on {weight.device}")
+    if bias is not None:
+        _refuse(bias.shape != weight.shape[:2] or bias.dtype != x.dtype or bias.device != x.device,
+                f"bias must be {tuple(weight.shape[:2])} {x.dtype} on {x.device}, got {tuple(bias.shape)} {bias.dtype} on {bias.device}")
+    ptr = _check_ptr(ptr, x)
+    _refuse(ptr.numel() != weight.shape[0] + 1, f"ptr must be [{weight.shape[0] + 1}] for {weight.shape[0]} groups, got [{ptr.numel()}]")
+    return _GroupedLinear.apply(x, weight, bias, ptr)
+
+
+class GroupedLinear(nn.Module):
+    """:func:`grouped_linear` with its parameters, each group's initialised as ``nn.Linear``'s."""
+
+    def __init__(self, num_groups: int, in_features: int, out_features: int, bias: bool = True, device=None, dtype=None):
+        super().__init__()
+        if min(num_groups, in_features, out_features) < 1:
+            raise ValueError(f"num_groups, in_features and out_features must be positive, got {num_groups}, {in_features}, {out_features}")
+        self.num_groups, self.in_features, self.out_features = num_groups, in_features, out_features
+        bound = in_features ** -0.5
+        self.weight = nn.Parameter(torch.empty(num_groups, out_features, in_features, device=device, dtype=dtype).uniform_(-bound, bound))
+        self.bias = nn.Parameter(torch.empty(num_groups, out_features, device=device, dtype=dtype).uniform_(-bound, bound)) if bias else None
+
+    def forward(self, x: torch.Tensor, ptr: torch.Tensor) -> torch.Tensor:
+        return grouped_linear(x, self.weight, ptr, self.bias)
+
+    def extra_repr(self) -> str:
+        return f"{self.num_groups}, {self.in_features}, {self.out_features}, bias={self.bias is not None}"
 
 
 # ---- group norm ----------------------------------------------------------------------------------------------------------------------

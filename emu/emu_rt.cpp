@@ -140,7 +140,7 @@ void launch(dim3 grid, dim3 block, size_t shmem, std::function<void()> body) {
     if (g_race) g_sh_dyn.assign(kSmem / 4 + 2, Shadow{0, 0, 0, 0});
   }
   const unsigned nthr = block.x * block.y * block.z;
-  if (block.y != 1 || block.z != 1 || grid.y != 1 || grid.z != 1 || nthr == 0 || nthr > 1024 || (nthr & 63) || shmem > kSmem) {
+  if (block.y != 1 || block.z != 1 || grid.z != 1 || nthr == 0 || nthr > 1024 || (nthr & 63) || shmem > kSmem) {
     fprintf(stderr, "dg_emu: unsupported launch shape grid (%u,%u,%u) block (%u,%u,%u) shmem %zu\n", grid.x, grid.y, grid.z, block.x,
             block.y, block.z, shmem);
     abort();
@@ -159,10 +159,10 @@ void launch(dim3 grid, dim3 block, size_t shmem, std::function<void()> body) {
   g_shmem = shmem;
   g_body = &body;
   g_blockDim = Idx{block.x, 1, 1};
-  g_gridDim = Idx{grid.x, 1, 1};
+  g_gridDim = Idx{grid.x, grid.y, 1};
   const unsigned nw = nthr / 64;
-  for (unsigned b = 0; b < grid.x; ++b) {
-    g_blockIdx = Idx{b, 0, 0};
+  for (unsigned b = 0; b < grid.x * grid.y; ++b) {
+    g_blockIdx = Idx{b % grid.x, b / grid.x, 0};
     ++g_epoch;                                   // (a new workgroup: nothing of the previous one's accesses counts)
     for (unsigned t = 0; t < nthr; ++t) {
       Lane& l = g_lanes[t];

@@ -198,6 +198,27 @@ static inline __attribute__((always_inline)) dg_emu_f32x4 __builtin_amdgcn_mfma_
     return d;
   }, dg_emu::Site{file_, line_, col_});
 }
+// v_mfma_f32_16x16x32_f16: the same layout
+typedef _Float16 dg_emu_f16x8 __attribute__((ext_vector_type(8)));
+static inline __attribute__((always_inline)) dg_emu_f32x4 __builtin_amdgcn_mfma_f32_16x16x32_f16(dg_emu_f16x8 a, dg_emu_f16x8 b, dg_emu_f32x4 c, int, int, int, const char* file_ = __builtin_FILE(), int line_ = __builtin_LINE(), int col_ = __builtin_COLUMN()) {
+  struct In { _Float16 a[8], b[8]; } in;
+  memcpy(in.a, &a, 16); memcpy(in.b, &b, 16);
+  return dg_emu_waveop(in, [c](int lane, const dg_emu::WaveBuf& w) {
+    dg_emu_f32x4 d = c;
+    const int n = lane & 15;
+    for (int r = 0; r < 4; ++r) {
+      const int m = 4 * (lane >> 4) + r;
+      double acc = d[r];
+      for (int kg = 0; kg < 4; ++kg) {
+        const In& A = DG_EMU_IN(In, w, 16 * kg + m);
+        const In& B = DG_EMU_IN(In, w, 16 * kg + n);
+        for (int e = 0; e < 8; ++e) acc += (double)(float)A.a[e] * (double)(float)B.b[e];
+      }
+      d[r] = (float)acc;
+    }
+    return d;
+  }, dg_emu::Site{file_, line_, col_});
+}
 // ds_read_b64_tr_b16: inside each group of 16 lanes the 16 x 4 fetched 16-bit elements form 4 rows of 16 (row j = the fetches of
 // lanes 4j .. 4j + 3, concatenated); lane l receives column l of the four rows
 typedef short dg_emu_s16x4 __attribute__((ext_vector_type(4)));

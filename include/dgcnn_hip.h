@@ -371,6 +371,22 @@ typedef struct dgcnn_adamw_args {
 } dgcnn_adamw_args;
 int dgcnn_adamw_step(const dgcnn_adamw_args* args, dgcnn_stream_t stream);
 
+/* Products grouped by type: rows ptr[e] .. ptr[e+1]-1 of x [rows, in_features] (row stride ldx elements) belong to group e,
+ *   y_i = weight_e x_i + bias_e     dx_i = weight_e^T dy_i     dweight_e = sum_i dy_i x_i^T     dbias_e = sum_i dy_i
+ * weight [groups, out_features, in_features], bias [groups, out_features] or NULL, y and dy [rows, out_features], dx [rows, in_features]
+ * (contiguous), everything of dtype.  ptr [groups + 1] int64 (device, ascending); groups may be empty (dweight and dbias 0); rows outside
+ * every group give 0 in y and dx.  (A ptr that does not ascend, or points outside [0, rows], gives unspecified values, never an access outside
+ * the tensors.)  _bwd: dx, dweight, dbias may each be NULL (dbias only with dweight); ws of dgcnn_grouped_linear_workspace_bytes. */
+typedef struct dgcnn_grouped_linear_args {
+  int64_t rows, ldx;
+  int32_t in_features, out_features, groups, dtype;
+  const void* x; const void* weight; const void* bias; const int64_t* ptr;
+} dgcnn_grouped_linear_args;
+int64_t dgcnn_grouped_linear_workspace_bytes(int64_t rows, int in_features, int out_features, int groups, int dtype);
+int dgcnn_grouped_linear_fwd(const dgcnn_grouped_linear_args* args, void* y, dgcnn_stream_t stream);
+int dgcnn_grouped_linear_bwd(const dgcnn_grouped_linear_args* args, const void* dy, void* dx, void* dweight, void* dbias, void* ws,
+                             dgcnn_stream_t stream);
+
 /* Group norm with an activation over rows of channels [rows, channels] (row-major, channels last), statistics for each segment of rows and each
  * group of channels / groups channels:  y = act((x - mean) / sqrt(var + eps) * weight + bias), var the mean squared difference.
  * ptr [segments + 1] int64 (device, ascending): segment s is rows ptr[s] .. ptr[s+1]-1, e.g. a batch's graphs; rows outside are set to
