@@ -23,7 +23,7 @@
 #define AW_THREADS 256
 #define AW_EPT 8           // consecutive elements of a thread
 #define AW_SPAN (AW_THREADS * AW_EPT)
-#define AW_TINY 7.7037197775489434e-34f      // 2^-110: a block whose largest value is below this is held as zeros (448 / it would overflow)
+#define AW_TINY 7.7037197775489434e-34f      // 2^-110: a block whose largest value is below this is held as zeros (448 times its inverse would overflow)
 
 struct DgAdamwTable {
   void* param[AW_TENSORS];
@@ -196,7 +196,7 @@ k_adamw(const DgAdamwTable t, const DgAdamwScalars byval, const DgAdamwScalars* 
       aw_store<DgF32>(static_cast<float*>(t.v[k]) + at, n, wide, v);
     } else {
       const float mtop = aw_block_max(m), rtop = aw_block_max(r);      // (elements behind the tensor's end are zeros)
-      const float minv = mtop > 0.f ? 448.f / mtop : 0.f, rinv = rtop > 0.f ? 448.f / rtop : 0.f;
+      const float minv = mtop > 0.f ? 1.f / mtop * 448.f : 0.f, rinv = rtop > 0.f ? 1.f / rtop * 448.f : 0.f;
       uint32_t wm[2] = {0, 0}, wv[2] = {0, 0};
 #pragma unroll
       for (int i = 0; i < AW_EPT; ++i) {
