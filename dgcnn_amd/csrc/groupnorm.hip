@@ -8,12 +8,12 @@
 // Bound: HBM (forward x in, y out; backward x and dy in, dx out).  The tensor is cut into CHUNKS of R rows, R such that a workgroup holds a
 // chunk in registers (NV vectors a thread), and every row is read once into registers, whatever the segments' lengths:
 //   * a segment of at most R rows belongs to one workgroup: read once, statistics over the registers (mean first, then the squares
-//     of the differences: no cancellation), written once;
+//     of the differences: no cancellation), written once (a form of the kernel for small tensors streams any length: L, not R, is where a segment counts as long);
 //   * a longer segment is the business of the chunks it spans: each leaves its partial (mean, M2) per group -- slot = chunk + segment, unique
 //     because (chunk, segment) pairs form a staircase -- and a second launch combines the partials of the segment (a few KB, from L2) and
 //     reads its chunk once more (from the last-level cache when the tensor fits it).
 // Lengths are known on the device alone, so both run in ONE launch (workgroups 0..segments-1 and the chunks behind them), and the second launch
-// is left out when the host knows that no segment can be longer than R (few rows, or equal lengths).  Nothing is summed by atomics: every
+// is left out when the host knows that no segment can be longer than L (few rows, or equal lengths).  Nothing is summed by atomics: every
 // sum has one order.
 // A thread keeps one column (VEC channels of one group) and every RY-th row; sums over a group go through one LDS slot a thread.
 // Statistics, partials and dw / db sums are fp32; y and dx are rounded once.
@@ -23,7 +23,8 @@
 // ... and at most, which is also how many vectors a group may be wide: 1024 threads leave 128 registers each, which wide vectors' arithmetic
 // (w, b, the sums of dw and db) spills
 static constexpr int gn_most(int vec) { return vec >= 4 ? 512 : 1024; }
-#define GN_WROWS 1024        // workgroups that keep dw / db sums (rows of partial sums)
+#define GN_WROWS 2048        // workgroups of a role that keep dw / db sums (rows of partial sums)
+#define GN_MAX_D 2048        // channels of a group
 
 struct DgGn {
   const void *x, *dy, *w, *b;
@@ -32,11 +33,12 @@ struct DgGn {
   float *mean, *rstd;            // [B][G]
   float *part;                   // [chunks + B][G][2]
   float *wpart;                  // [wrows][2][C]
-  int64_t N, per;
+  float *ac;                     // backward, long segments: [B][G][2], the two means
+  int64_t N, per, L;             // a segment of more than L rows is split over the workgroups of its chunks
   int B, C, G, D, DV, Gt, CVt, RY, R, P;      // D channels = DV vectors a group; Gt groups (CVt vectors) a workgroup; R = RY * NV rows a chunk; P lanes sum a group
   int nseg;                      // workgroups that own whole segments
   int nchunk, cgrid;             // chunks; workgroups that walk them (0: no segment is split)
-  int wdt, act, relaxed;         // type of w and b; activation; 1: a long segment is streamed by its workgroup (no second launch)
+  int wdt, act;                  // type of w and b; activation
   float eps;
 };
 
@@ -119,7 +121,7 @@ __device__ __forceinline__ void gn_range(const DgGn& a, int s, int64_t& lo, int6
 }
 // the segment that row r lies in (-1: in front of the first; B: behind the last), found by the whole wave: 64 probes a step
 __device__ __forceinline__ int gn_find(const DgGn& a, int64_t r) {
-  if (!a.ptr) return (int)(r / a.per);
+  if (!a.ptr) return (r | a.per) >> 31 ? (int)(r / a.per) : (int)((unsigned)r / (unsigned)a.per);
   const int lane = threadIdx.x & 63;
   int64_t lo = 0, hi = a.B + 1;
   while (lo < hi) {
@@ -132,6 +134,9 @@ __device__ __forceinline__ int gn_find(const DgGn& a, int64_t r) {
   return (int)lo - 1;
 }
 
+template <int CTRL> __device__ __forceinline__ float gn_dpp(float x) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xF, 0xF, true));
+}
 // ---- sums over a group -----------------------------------------------------------------------------------------------------------
 struct GnLds { float red[2][1024]; float stat[2][1024]; };
 struct GnLane {
@@ -139,16 +144,26 @@ struct GnLane {
   unsigned off;              // of the thread's vector in row block 0
   bool on;                   // the thread owns a column (else r lies behind every row)
 };
+// x summed over P = 1, 4, 16 or 64 neighbouring lanes, the sum in all of them
+__device__ __forceinline__ float gn_lanes(float x, int P) {
+  if (P >= 4) { x += gn_dpp<0xB1>(x); x += gn_dpp<0x4E>(x); }              // quad_perm [1 0 3 2], [2 3 0 1]
+  if (P >= 16) { x += gn_dpp<0x124>(x); x += gn_dpp<0x128>(x); }           // row_ror 4, 8
+  if (P >= 64) { x += __shfl_xor(x, 16); x += __shfl_xor(x, 32); }
+  return x;
+}
 // every thread's u (and v) summed over its group -> L.stat[0/1][group].  Two barriers a sum; the first one of the next sum is what keeps this one's
-// results in place until everyone has read them.
+// results in place until everyone has read them.  P lanes add a group's slots: few enough that each has several reads in flight.
 template <bool TWO> __device__ __forceinline__ void gn_sum(const DgGn& a, GnLds& L, const GnLane& me, int gn, float u, float v) {
   if (me.on) { L.red[0][me.slot] = u; if (TWO) L.red[1][me.slot] = v; }
   __syncthreads();
   const int items = a.RY * a.DV, g = me.t / a.P, l = me.t & (a.P - 1);
   float su = 0.f, sv = 0.f;
-  if (g < gn)
+  if (g < gn) {
+#pragma unroll 4
     for (int j = l; j < items; j += a.P) { su += L.red[0][g * items + j]; if (TWO) sv += L.red[1][g * items + j]; }
-  for (int o = a.P >> 1; o; o >>= 1) { su += __shfl_xor(su, o); if (TWO) sv += __shfl_xor(sv, o); }
+  }
+  su = gn_lanes(su, a.P);
+  if (TWO) sv = gn_lanes(sv, a.P);
   if (g < gn && l == 0) { L.stat[0][g] = su; if (TWO) L.stat[1][g] = sv; }
   __syncthreads();
 }
@@ -158,8 +173,26 @@ template <class D, int VEC> __device__ __forceinline__ void gn_zero_rows(const D
     if (me.r < hi - at) dg_store<D, VEC>(static_cast<typename D::S*>(a.out) + at * a.C + me.off, dg_zero<D, VEC>());
 }
 
+template <int VEC> __device__ __forceinline__ void gn_load_w(const void* p, int dt, bool on, int ch, float absent, float* w) {
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) w[i] = absent;
+  if (!p || !on) return;
+  if (dt == DGCNN_F32) {      // (the branch outside the elements: their loads become one)
+    const float* const q = static_cast<const float*>(p) + ch;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) w[i] = q[i];
+  } else if (dt == DGCNN_BF16) {
+    const uint16_t* const q = static_cast<const uint16_t*>(p) + ch;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) w[i] = DgBF16::to(q[i]);
+  } else {
+    const uint16_t* const q = static_cast<const uint16_t*>(p) + ch;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) w[i] = DgF16::to(q[i]);
+  }
+}
+
 #define GN_SETUP()                                                                                                     \
-  __shared__ GnLds L;                                                                                                  \
   const int g0 = blockIdx.y * a.Gt, gn = min(a.Gt, a.G - g0);                                                          \
   GnLane me;                                                                                                           \
   me.t = threadIdx.x; me.r = me.t / a.CVt; me.c = me.t - me.r * a.CVt; me.g = me.c / a.DV;                             \
@@ -172,10 +205,8 @@ template <class D, int VEC> __device__ __forceinline__ void gn_zero_rows(const D
   const S* const x = static_cast<const S*>(a.x);                                                                       \
   S* const out = static_cast<S*>(a.out);                                                                               \
   float w[VEC], b[VEC];                                                                                                \
-  _Pragma("unroll") for (int i = 0; i < VEC; ++i) {                                                                    \
-    w[i] = a.w && me.on ? dg_load_as(a.w, ch + i, a.wdt) : 1.f;                                                        \
-    b[i] = a.b && me.on ? dg_load_as(a.b, ch + i, a.wdt) : 0.f;                                                        \
-  }                                                                                                                    \
+  gn_load_w<VEC>(a.w, a.wdt, me.on, ch, 1.f, w);                                                                       \
+  gn_load_w<VEC>(a.b, a.wdt, me.on, ch, 0.f, b);                                                                       \
   (void)x; (void)out; (void)b; (void)ch
 
 // Rows are addressed as (uniform base of the row block i RY) + (the thread's own 32-bit offset): a 64-bit address a row and thread would take
@@ -187,13 +218,18 @@ template <class D, int VEC, int NV> __device__ __forceinline__ void gn_load(cons
     if (me.r < left - i * a.RY) v[i] = dg_load<D, VEC>(p + (at + (int64_t)i * a.RY) * a.C + me.off);
   }
 }
-__device__ __forceinline__ int gn_left(const DgGn& a, int64_t at, int64_t hi) { return (int)min(hi - at, (int64_t)a.R); }
+// What does not fit the registers passes through them R rows at a time: f(at, left) for each piece
+template <class F> __device__ __forceinline__ void gn_pieces(const DgGn& a, int64_t lo, int64_t hi, F f) {
+#pragma unroll 1
+  for (int64_t at = lo; at < hi; at += a.R) f(at, (int)min(hi - at, (int64_t)a.R));
+}
 
-template <class D, int VEC> __device__ __forceinline__ DgRaw<D, VEC> gn_apply(const DgGn& a, const DgRaw<D, VEC>& v, float mu, float rs, const float* w, const float* b) {
+// x - mu is kept apart from the scale: a constant segment gives exactly b, and a large mean cancels before anything is rounded.  rw = rstd * w.
+template <class D, int VEC> __device__ __forceinline__ DgRaw<D, VEC> gn_apply(const DgGn& a, const DgRaw<D, VEC>& v, float mu, const float* rw, const float* b) {
   float z[VEC];
   DgRaw<D, VEC> o;
 #pragma unroll
-  for (int e = 0; e < VEC; ++e) z[e] = (v.get(e) - mu) * rs * w[e] + b[e];
+  for (int e = 0; e < VEC; ++e) z[e] = __builtin_fmaf(v.get(e) - mu, rw[e], b[e]);
   gn_act<VEC>(a.act, z);
 #pragma unroll
   for (int e = 0; e < VEC; ++e) o.set(e, z[e]);
@@ -221,7 +257,7 @@ struct GnWork {
         s = next++; slot = -1;
         gn_range(a, s, lo, hi);
         if (lo == hi) { empty(s); continue; }
-        if (hi - lo > a.R && !a.relaxed) continue;
+        if (hi - lo > a.L) continue;
         return true;
       }
       if (next > end) {
@@ -234,7 +270,7 @@ struct GnWork {
       s = next; slot = k + s;
       next = s < end ? end : end + 1;      // (a segment longer than a chunk is the chunk's first or its last)
       gn_range(a, s, lo, hi);
-      if (hi - lo <= a.R) continue;
+      if (hi - lo <= a.L) continue;
       lo = max(lo, (int64_t)k * a.R); hi = min(hi, (int64_t)(k + 1) * a.R);
       if (lo < hi) return true;
     }
@@ -250,9 +286,10 @@ template <class D, int VEC> __device__ __forceinline__ void gn_clear(const DgGn&
 
 // forward: whole segments, and the partial moments of the chunks of long ones.  More than R rows (a few long segments, no second launch) pass
 // through the registers piece by piece, read again for each of the three passes.
-template <class D, int VEC, int NV>
+template <class D, int VEC, int NV, bool STREAM>
 __global__ void __launch_bounds__(gn_most(VEC))
 k_gn_fwd(const DgGn a) {
+  __shared__ GnLds L;
   GN_SETUP();
   DgRaw<D, VEC> v[NV];
   gn_clear<D, VEC>(a, me);
@@ -260,32 +297,49 @@ k_gn_fwd(const DgGn a) {
   while (it.fetch(a, [&](int s) {
     if (me.t < gn) { a.mean[(int64_t)s * a.G + g0 + me.t] = 0.f; a.rstd[(int64_t)s * a.G + g0 + me.t] = 0.f; }
   })) {
-    const bool again = it.hi - it.lo > a.R;
+    const int left = (int)min(it.hi - it.lo, (int64_t)a.R);
     const float n = (float)(it.hi - it.lo) * (float)a.D;
     float sum = 0.f, sq = 0.f;
-    for (int64_t at = it.lo; at < it.hi; at += a.R) {
-      const int left = gn_left(a, at, it.hi);
-      gn_load<D, VEC, NV>(a, me, x, at, left, v);
+    if constexpr (!STREAM) {
+      gn_load<D, VEC, NV>(a, me, x, it.lo, left, v);
 #pragma unroll
       for (int i = 0; i < NV; ++i)
 #pragma unroll
         for (int e = 0; e < VEC; ++e) sum += v[i].get(e);
+    } else {
+      gn_pieces(a, it.lo, it.hi, [&](int64_t at, int left) {
+        DgRaw<D, VEC> u[NV];
+        gn_load<D, VEC, NV>(a, me, x, at, left, u);
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) sum += u[i].get(e);
+      });
     }
     gn_sum<false>(a, L, me, gn, sum, 0.f);
-    dg_hide<D, VEC, NV>(v);
+    if constexpr (!STREAM) dg_hide<D, VEC, NV>(v);
     const float mu = me.on ? L.stat[0][me.g] / n : 0.f;      // (divided: a constant segment's mean is the constant, its squares' sum 0)
-    for (int64_t at = it.lo; at < it.hi; at += a.R) {
-      const int left = gn_left(a, at, it.hi);
-      if (again) gn_load<D, VEC, NV>(a, me, x, at, left, v);
+    if constexpr (!STREAM) {
 #pragma unroll
       for (int i = 0; i < NV; ++i)
         if (me.r < left - i * a.RY) {
 #pragma unroll
           for (int e = 0; e < VEC; ++e) { const float d = v[i].get(e) - mu; sq += d * d; }
         }
+    } else {
+      gn_pieces(a, it.lo, it.hi, [&](int64_t at, int left) {
+        DgRaw<D, VEC> u[NV];
+        gn_load<D, VEC, NV>(a, me, x, at, left, u);
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+          if (me.r < left - i * a.RY) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) { const float d = u[i].get(e) - mu; sq += d * d; }
+          }
+      });
     }
     gn_sum<false>(a, L, me, gn, sq, 0.f);
-    dg_hide<D, VEC, NV>(v);
+    if constexpr (!STREAM) dg_hide<D, VEC, NV>(v);
     const bool first = me.r == 0 && me.c == me.g * a.DV;      // one thread of each group
     if (it.slot >= 0) {
       if (first) {
@@ -296,104 +350,132 @@ k_gn_fwd(const DgGn a) {
     }
     const float rs = me.on ? 1.f / sqrtf(L.stat[0][me.g] / n + a.eps) : 0.f;
     if (first) { a.mean[(int64_t)it.s * a.G + g0 + me.g] = mu; a.rstd[(int64_t)it.s * a.G + g0 + me.g] = rs; }
-    for (int64_t at = it.lo; at < it.hi; at += a.R) {
-      const int left = gn_left(a, at, it.hi);
-      if (again) gn_load<D, VEC, NV>(a, me, x, at, left, v);
+    float rw[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) rw[e] = rs * w[e];
+    if constexpr (!STREAM) {
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        if (me.r < left - i * a.RY) dg_store<D, VEC>(out + (at + (int64_t)i * a.RY) * a.C + me.off, gn_apply<D, VEC>(a, v[i], mu, rs, w, b));
+        if (me.r < left - i * a.RY) dg_store<D, VEC>(out + (it.lo + (int64_t)i * a.RY) * a.C + me.off, gn_apply<D, VEC>(a, v[i], mu, rw, b));
         GN_FENCE();
       }
+    } else {
+      gn_pieces(a, it.lo, it.hi, [&](int64_t at, int left) {
+        DgRaw<D, VEC> u[NV];
+        gn_load<D, VEC, NV>(a, me, x, at, left, u);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+          if (me.r < left - i * a.RY) dg_store<D, VEC>(out + (at + (int64_t)i * a.RY) * a.C + me.off, gn_apply<D, VEC>(a, u[i], mu, rw, b));
+          GN_FENCE();
+        }
+      });
     }
   }
 }
 
-// the chunks of long segments: partial moments -> mean, rstd -> y; rows outside every segment -> 0
+// ---- long segments: the partials of a segment's chunks, then its rows once more -----------------------------------------------------
+// 16 lanes a (segment, group).  Forward: mean = sum n_i mean_i / n, M2 = sum M2_i + n_i (mean_i - mean)^2 -> mean, rstd.  Backward: the two means -> ac.
+template <bool BWD> __device__ __forceinline__ void gn_join(const DgGn& a, int64_t item) {
+  const int l = threadIdx.x & 15, s = (int)(item / a.G), g = (int)(item % a.G);
+  int64_t lo = 0, hi = 0;
+  if (s < a.B) {
+    if (a.ptr) { lo = min(max(a.ptr[s], (int64_t)0), a.N); hi = min(max(a.ptr[s + 1], lo), a.N); }
+    else { lo = (int64_t)s * a.per; hi = lo + a.per; }
+  }
+  const bool on = hi - lo > a.L;
+  const int k0 = (int)(lo / a.R), n = on ? (int)((hi - 1) / a.R) - k0 + 1 : 0;
+  const float* const p = a.part + ((int64_t)(k0 + s) * a.G + g) * 2;
+  const float rows = (float)(hi - lo);
+  float u = 0.f, v = 0.f;
+  if (BWD) {
+#pragma unroll 4
+    for (int i = l; i < n; i += 16) { u += p[(int64_t)i * a.G * 2]; v += p[(int64_t)i * a.G * 2 + 1]; }
+    u = gn_lanes(u, 16); v = gn_lanes(v, 16);
+    if (on && l == 0) {
+      a.ac[((int64_t)s * a.G + g) * 2] = u / (rows * (float)a.D);
+      a.ac[((int64_t)s * a.G + g) * 2 + 1] = v / (rows * (float)a.D);
+    }
+    return;
+  }
+#pragma unroll 4
+  for (int i = l; i < n; i += 16)
+    u += p[(int64_t)i * a.G * 2] * (float)(min((int64_t)(k0 + i + 1) * a.R, hi) - max((int64_t)(k0 + i) * a.R, lo));
+  u = gn_lanes(u, 16);
+  const float m = u / rows;
+#pragma unroll 4
+  for (int i = l; i < n; i += 16) {
+    const float d = p[(int64_t)i * a.G * 2] - m;
+    v += p[(int64_t)i * a.G * 2 + 1] + (float)(min((int64_t)(k0 + i + 1) * a.R, hi) - max((int64_t)(k0 + i) * a.R, lo)) * (float)a.D * d * d;
+  }
+  v = gn_lanes(v, 16);
+  if (on && l == 0) {
+    a.mean[(int64_t)s * a.G + g] = m;
+    a.rstd[(int64_t)s * a.G + g] = 1.f / sqrtf(v / rows / (float)a.D + a.eps);
+  }
+}
+__global__ void __launch_bounds__(256) k_gn_join(const DgGn a) { gn_join<false>(a, (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4)); }
+
+// rows [at0, at1) of long segment s; ROWS(at, left) for each R of them
+template <class F> __device__ __forceinline__ void gn_long_rows(const DgGn& a, int k, F rows) {
+  const int64_t r0 = (int64_t)k * a.R, r1 = min(r0 + a.R, a.N);
+  const int s0 = max(gn_find(a, r0), 0), s1 = min(gn_find(a, r1 - 1), a.B - 1);
+  for (int s = s0; s <= s1; s = s < s1 ? s1 : s1 + 1) {
+    int64_t lo, hi;
+    gn_range(a, s, lo, hi);
+    if (hi - lo <= a.L) continue;
+    lo = max(lo, r0); hi = min(hi, r1);
+    if (lo < hi) rows(s, lo, (int)(hi - lo));
+  }
+}
+// the chunk's rows that lie in no segment -> 0
+template <class D, int VEC> __device__ __forceinline__ void gn_clear_chunk(const DgGn& a, const GnLane& me, int k) {
+  if (!a.ptr) return;
+  const int64_t r0 = (int64_t)k * a.R, r1 = min(r0 + a.R, a.N);
+  int64_t lo, hi, u;
+  gn_range(a, 0, lo, u);
+  gn_range(a, a.B - 1, u, hi);
+  if (r0 < lo) gn_zero_rows<D, VEC>(a, me, r0, min(lo, r1));
+  if (hi < r1) gn_zero_rows<D, VEC>(a, me, max(hi, r0), r1);
+}
 template <class D, int VEC, int NV>
 __global__ void __launch_bounds__(gn_most(VEC))
 k_gn_fwd_long(const DgGn a) {
   GN_SETUP();
-  for (int k = blockIdx.x; k < a.nchunk; k += gridDim.x) {
-    const int64_t r0 = (int64_t)k * a.R, r1 = min(r0 + a.R, a.N);
-    const int f0 = gn_find(a, r0), f1 = gn_find(a, r1 - 1);
-    if (f0 < 0 || f1 >= a.B) {
-      int64_t lo, hi, u;
-      gn_range(a, 0, lo, u);
-      gn_range(a, a.B - 1, u, hi);
-      if (f0 < 0) gn_zero_rows<D, VEC>(a, me, r0, min(lo, r1));
-      if (f1 >= a.B) gn_zero_rows<D, VEC>(a, me, max(hi, r0), r1);
-    }
-    const int s0 = max(f0, 0), s1 = min(f1, a.B - 1);
-    for (int s = s0; s <= s1; s = s < s1 ? s1 : s1 + 1) {
-      int64_t lo, hi;
-      gn_range(a, s, lo, hi);
-      if (hi - lo <= a.R) continue;
-      const int64_t a0 = max(lo, r0), a1 = min(hi, r1);
-      if (a0 >= a1) continue;
-      const int left = (int)(a1 - a0);
-      DgRaw<D, VEC> v[NV];
-      gn_load<D, VEC, NV>(a, me, x, a0, left, v);      // (in flight while the partials are combined)
-      // mean = sum n_i mean_i / n;   M2 = sum M2_i + n_i (mean_i - mean)^2
-      const int k0 = (int)(lo / a.R), k1 = (int)((hi - 1) / a.R), g = me.t / a.P, l = me.t & (a.P - 1);
-      const float* const p = a.part + ((int64_t)(k0 + s) * a.G + g0 + g) * 2;
-      const float n = (float)(hi - lo);
-      float m = 0.f, q = 0.f;
-      if (g < gn)
-        for (int i = l; i <= k1 - k0; i += a.P)
-          m += p[(int64_t)i * a.G * 2] * (float)(min((int64_t)(k0 + i + 1) * a.R, hi) - max((int64_t)(k0 + i) * a.R, lo));
-      for (int o = a.P >> 1; o; o >>= 1) m += __shfl_xor(m, o);
-      m /= n;
-      if (g < gn)
-        for (int i = l; i <= k1 - k0; i += a.P) {
-          const float d = p[(int64_t)i * a.G * 2] - m;
-          q += p[(int64_t)i * a.G * 2 + 1] + (float)(min((int64_t)(k0 + i + 1) * a.R, hi) - max((int64_t)(k0 + i) * a.R, lo)) * (float)a.D * d * d;
-        }
-      for (int o = a.P >> 1; o; o >>= 1) q += __shfl_xor(q, o);
-      if (g < gn && l == 0) {
-        const float rs = 1.f / sqrtf(q / n / (float)a.D + a.eps);
-        L.stat[0][g] = m; L.stat[1][g] = rs;
-        if (k == k0) { a.mean[(int64_t)s * a.G + g0 + g] = m; a.rstd[(int64_t)s * a.G + g0 + g] = rs; }
-      }
-      __syncthreads();
-      const float mu = me.on ? L.stat[0][me.g] : 0.f, rs = me.on ? L.stat[1][me.g] : 0.f;
+  gn_clear_chunk<D, VEC>(a, me, blockIdx.x);
+  gn_long_rows(a, blockIdx.x, [&](int s, int64_t at, int left) {
+    DgRaw<D, VEC> v[NV];
+    gn_load<D, VEC, NV>(a, me, x, at, left, v);
+    const float mu = me.on ? a.mean[(int64_t)s * a.G + g0 + me.g] : 0.f, rs = me.on ? a.rstd[(int64_t)s * a.G + g0 + me.g] : 0.f;
+    float rw[VEC];
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        if (me.r < left - i * a.RY) dg_store<D, VEC>(out + (a0 + (int64_t)i * a.RY) * a.C + me.off, gn_apply<D, VEC>(a, v[i], mu, rs, w, b));
-        GN_FENCE();
-      }
-      __syncthreads();
+    for (int e = 0; e < VEC; ++e) rw[e] = rs * w[e];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      if (me.r < left - i * a.RY) dg_store<D, VEC>(out + (at + (int64_t)i * a.RY) * a.C + me.off, gn_apply<D, VEC>(a, v[i], mu, rw, b));
+      GN_FENCE();
     }
-  }
+  });
 }
 
 // ---- backward --------------------------------------------------------------------------------------------------------------------
-// h and q of one vector
-template <class D, int VEC> __device__ __forceinline__ void gn_hq(const DgGn& a, const DgRaw<D, VEC>& x, const DgRaw<D, VEC>& dy, float mu, float rs, const float* w, const float* b, float* h, float* q) {
+// With t = x - mu, h = t rstd:  q = dy act'(t rw + b);  over a segment's rows, per channel, sq = sum q and sqt = sum q t give everything: db = sq, dw = rstd sqt,
+// and over a group's channels a = sum w sq / n, c = rstd sum w sqt / n.   dx = rw q - rstd a - t (rstd^2 c) = rw q - A - t B
+template <class D, int VEC> __device__ __forceinline__ void gn_q(const DgGn& a, const DgRaw<D, VEC>& x, const DgRaw<D, VEC>& dy, float mu, const float* rw, const float* b, float* q) {
 #pragma unroll
-  for (int e = 0; e < VEC; ++e) { h[e] = (x.get(e) - mu) * rs; q[e] = h[e] * w[e] + b[e]; }
+  for (int e = 0; e < VEC; ++e) q[e] = __builtin_fmaf(x.get(e) - mu, rw[e], b[e]);
   gn_slope<VEC>(a.act, q);
 #pragma unroll
   for (int e = 0; e < VEC; ++e) q[e] *= dy.get(e);
 }
-template <class D, int VEC> __device__ __forceinline__ DgRaw<D, VEC> gn_dx(const DgGn& a, const DgRaw<D, VEC>& x, const DgRaw<D, VEC>& dy, float mu, float rs, const float* w, const float* b, float am, float cm) {
-  float h[VEC], q[VEC];
-  gn_hq<D, VEC>(a, x, dy, mu, rs, w, b, h, q);
+template <class D, int VEC> __device__ __forceinline__ DgRaw<D, VEC> gn_dx(const DgRaw<D, VEC>& x, float mu, const float* q, const float* rw, float A, float B) {
   DgRaw<D, VEC> o;
 #pragma unroll
-  for (int e = 0; e < VEC; ++e) o.set(e, rs * (q[e] * w[e] - am - h[e] * cm));
+  for (int e = 0; e < VEC; ++e) o.set(e, __builtin_fmaf(q[e], rw[e], -__builtin_fmaf(x.get(e) - mu, B, A)));
   return o;
 }
-// one vector into the thread's sums
-template <class D, int VEC> __device__ __forceinline__ void gn_add(const DgGn& a, const DgRaw<D, VEC>& x, const DgRaw<D, VEC>& dy, float mu, float rs, const float* w, const float* b, float* dw, float* db, float& s1, float& s2) {
-  float h[VEC], q[VEC];
-  gn_hq<D, VEC>(a, x, dy, mu, rs, w, b, h, q);
+template <class D, int VEC> __device__ __forceinline__ void gn_add(const DgRaw<D, VEC>& x, float mu, const float* q, float* sq, float* sqt) {
 #pragma unroll
-  for (int e = 0; e < VEC; ++e) {
-    db[e] += q[e];
-    dw[e] += q[e] * h[e];
-    const float qw = q[e] * w[e];
-    s1 += qw; s2 += qw * h[e];
-  }
+  for (int e = 0; e < VEC; ++e) { sq[e] += q[e]; sqt[e] = __builtin_fmaf(q[e], x.get(e) - mu, sqt[e]); }
 }
 // the workgroup's dw, db sums -> its row of wpart
 template <int VEC> __device__ __forceinline__ void gn_put_w(const DgGn& a, GnLds& L, const GnLane& me, int gn, int ch, const float* dw, const float* db) {
@@ -412,30 +494,58 @@ template <int VEC> __device__ __forceinline__ void gn_put_w(const DgGn& a, GnLds
 }
 
 // backward: whole segments (each workgroup walks a contiguous share of them), and the partial sums of the chunks of long ones
-template <class D, int VEC, int NV>
+template <class D, int VEC, int NV, bool STREAM>
 __global__ void __launch_bounds__(gn_most(VEC))
 k_gn_bwd(const DgGn a) {
+  __shared__ GnLds L;
   GN_SETUP();
   const S* const dy = static_cast<const S*>(a.dy);
-  DgRaw<D, VEC> v[NV], d[NV];
   float dw[VEC], db[VEC];
 #pragma unroll
   for (int e = 0; e < VEC; ++e) dw[e] = db[e] = 0.f;
   gn_clear<D, VEC>(a, me);
   GnWork it(a);
   while (it.fetch(a, [](int) {})) {
-    const bool again = it.hi - it.lo > a.R;
+    const int left = (int)min(it.hi - it.lo, (int64_t)a.R);
     const float inv_n = 1.f / ((float)(it.hi - it.lo) * (float)a.D);
-    float mu = me.on ? a.mean[(int64_t)it.s * a.G + g0 + me.g] : 0.f;
+    const float mu = me.on ? a.mean[(int64_t)it.s * a.G + g0 + me.g] : 0.f;
     const float rs = me.on ? a.rstd[(int64_t)it.s * a.G + g0 + me.g] : 0.f;
-    float s1 = 0.f, s2 = 0.f;
-    for (int64_t at = it.lo; at < it.hi; at += a.R) {
-      const int left = gn_left(a, at, it.hi);
-      gn_load<D, VEC, NV>(a, me, x, at, left, v);
-      gn_load<D, VEC, NV>(a, me, dy, at, left, d);
+    float rw[VEC], sq[VEC], sqt[VEC];
 #pragma unroll
-      for (int i = 0; i < NV; ++i)
-        { if (me.r < left - i * a.RY) gn_add<D, VEC>(a, v[i], d[i], mu, rs, w, b, dw, db, s1, s2); GN_FENCE(); }
+    for (int e = 0; e < VEC; ++e) { rw[e] = rs * w[e]; sq[e] = sqt[e] = 0.f; }
+    DgRaw<D, VEC> v[NV];
+    float q[NV][VEC];      // (kept over the sum: the activation's slope costs more than anything else here)
+    if constexpr (!STREAM) {
+      DgRaw<D, VEC> d[NV];
+      gn_load<D, VEC, NV>(a, me, x, it.lo, left, v);
+      gn_load<D, VEC, NV>(a, me, dy, it.lo, left, d);
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        if (i * a.RY >= left) continue;      // (uniform: whole row blocks that are not there; a missing row of the last one has dy = 0, q = 0)
+        gn_q<D, VEC>(a, v[i], d[i], mu, rw, b, q[i]);
+        gn_add<D, VEC>(v[i], mu, q[i], sq, sqt);
+        GN_FENCE();
+      }
+    } else {
+      gn_pieces(a, it.lo, it.hi, [&](int64_t at, int left) {
+        DgRaw<D, VEC> d[NV];
+        gn_load<D, VEC, NV>(a, me, x, at, left, v);
+        gn_load<D, VEC, NV>(a, me, dy, at, left, d);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+          if (me.r < left - i * a.RY) {
+            gn_q<D, VEC>(a, v[i], d[i], mu, rw, b, q[i]);
+            gn_add<D, VEC>(v[i], mu, q[i], sq, sqt);
+          }
+          GN_FENCE();
+        }
+      });
+    }
+    float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      s1 += w[e] * sq[e]; s2 += rw[e] * sqt[e];
+      db[e] += sq[e]; dw[e] += rs * sqt[e];
     }
     gn_sum<true>(a, L, me, gn, s1, s2);
     if (it.slot >= 0) {
@@ -445,18 +555,28 @@ k_gn_bwd(const DgGn a) {
       }
       continue;
     }
-    dg_hide<D, VEC, NV>(v);      // (h and q are computed again: held over the sum they take twice the registers of x and dy)
-    dg_hide<D, VEC, NV>(d);
-    DG_OPAQUE_V(mu);
-    const float am = me.on ? L.stat[0][me.g] * inv_n : 0.f, cm = me.on ? L.stat[1][me.g] * inv_n : 0.f;
-    for (int64_t at = it.lo; at < it.hi; at += a.R) {
-      const int left = gn_left(a, at, it.hi);
-      if (again) { gn_load<D, VEC, NV>(a, me, x, at, left, v); gn_load<D, VEC, NV>(a, me, dy, at, left, d); }
+    const float A = me.on ? rs * (L.stat[0][me.g] * inv_n) : 0.f, B = me.on ? rs * rs * (L.stat[1][me.g] * inv_n) : 0.f;
+    if constexpr (!STREAM) {
+      dg_hide<D, VEC, NV>(v);
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        if (me.r < left - i * a.RY) dg_store<D, VEC>(out + (at + (int64_t)i * a.RY) * a.C + me.off, gn_dx<D, VEC>(a, v[i], d[i], mu, rs, w, b, am, cm));
+        if (me.r < left - i * a.RY) dg_store<D, VEC>(out + (it.lo + (int64_t)i * a.RY) * a.C + me.off, gn_dx<D, VEC>(v[i], mu, q[i], rw, A, B));
         GN_FENCE();
       }
+    } else {
+      gn_pieces(a, it.lo, it.hi, [&](int64_t at, int left) {
+        DgRaw<D, VEC> d[NV];
+        gn_load<D, VEC, NV>(a, me, x, at, left, v);
+        gn_load<D, VEC, NV>(a, me, dy, at, left, d);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+          if (me.r < left - i * a.RY) {
+            gn_q<D, VEC>(a, v[i], d[i], mu, rw, b, q[i]);
+            dg_store<D, VEC>(out + (at + (int64_t)i * a.RY) * a.C + me.off, gn_dx<D, VEC>(v[i], mu, q[i], rw, A, B));
+          }
+          GN_FENCE();
+        }
+      });
     }
   }
   if (a.wpart) gn_put_w<VEC>(a, L, me, gn, ch, dw, db);
@@ -467,115 +587,104 @@ __global__ void __launch_bounds__(gn_most(VEC))
 k_gn_bwd_long(const DgGn a) {
   GN_SETUP();
   const S* const dy = static_cast<const S*>(a.dy);
-  for (int k = blockIdx.x; k < a.nchunk; k += gridDim.x) {
-    const int64_t r0 = (int64_t)k * a.R, r1 = min(r0 + a.R, a.N);
-    const int f0 = gn_find(a, r0), f1 = gn_find(a, r1 - 1);
-    if (f0 < 0 || f1 >= a.B) {
-      int64_t lo, hi, u;
-      gn_range(a, 0, lo, u);
-      gn_range(a, a.B - 1, u, hi);
-      if (f0 < 0) gn_zero_rows<D, VEC>(a, me, r0, min(lo, r1));
-      if (f1 >= a.B) gn_zero_rows<D, VEC>(a, me, max(hi, r0), r1);
-    }
-    const int s0 = max(f0, 0), s1 = min(f1, a.B - 1);
-    for (int s = s0; s <= s1; s = s < s1 ? s1 : s1 + 1) {
-      int64_t lo, hi;
-      gn_range(a, s, lo, hi);
-      if (hi - lo <= a.R) continue;
-      const int64_t a0 = max(lo, r0), a1 = min(hi, r1);
-      if (a0 >= a1) continue;
-      const int left = (int)(a1 - a0);
-      DgRaw<D, VEC> v[NV], d[NV];
-      gn_load<D, VEC, NV>(a, me, x, a0, left, v);
-      gn_load<D, VEC, NV>(a, me, dy, a0, left, d);
-      const int k0 = (int)(lo / a.R), k1 = (int)((hi - 1) / a.R), g = me.t / a.P, l = me.t & (a.P - 1);
-      const float* const p = a.part + ((int64_t)(k0 + s) * a.G + g0 + g) * 2;
-      float u1 = 0.f, u2 = 0.f;
-      if (g < gn)
-        for (int i = l; i <= k1 - k0; i += a.P) { u1 += p[(int64_t)i * a.G * 2]; u2 += p[(int64_t)i * a.G * 2 + 1]; }
-      for (int o = a.P >> 1; o; o >>= 1) { u1 += __shfl_xor(u1, o); u2 += __shfl_xor(u2, o); }
-      if (g < gn && l == 0) {
-        const float inv_n = 1.f / ((float)(hi - lo) * (float)a.D);
-        L.stat[0][g] = u1 * inv_n; L.stat[1][g] = u2 * inv_n;
-      }
-      __syncthreads();
-      const float am = me.on ? L.stat[0][me.g] : 0.f, cm = me.on ? L.stat[1][me.g] : 0.f;
-      const float mu = me.on ? a.mean[(int64_t)s * a.G + g0 + me.g] : 0.f, rs = me.on ? a.rstd[(int64_t)s * a.G + g0 + me.g] : 0.f;
+  gn_clear_chunk<D, VEC>(a, me, blockIdx.x);
+  gn_long_rows(a, blockIdx.x, [&](int s, int64_t at, int left) {
+    DgRaw<D, VEC> v[NV], d[NV];
+    gn_load<D, VEC, NV>(a, me, x, at, left, v);
+    gn_load<D, VEC, NV>(a, me, dy, at, left, d);
+    const int64_t sg = (int64_t)s * a.G + g0 + me.g;
+    const float mu = me.on ? a.mean[sg] : 0.f, rs = me.on ? a.rstd[sg] : 0.f;
+    const float A = me.on ? rs * a.ac[2 * sg] : 0.f, B = me.on ? rs * rs * a.ac[2 * sg + 1] : 0.f;
+    float rw[VEC];
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        if (me.r < left - i * a.RY) dg_store<D, VEC>(out + (a0 + (int64_t)i * a.RY) * a.C + me.off, gn_dx<D, VEC>(a, v[i], d[i], mu, rs, w, b, am, cm));
-        GN_FENCE();
+    for (int e = 0; e < VEC; ++e) rw[e] = rs * w[e];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      if (me.r < left - i * a.RY) {
+        float q[VEC];
+        gn_q<D, VEC>(a, v[i], d[i], mu, rw, b, q);
+        dg_store<D, VEC>(out + (at + (int64_t)i * a.RY) * a.C + me.off, gn_dx<D, VEC>(v[i], mu, q, rw, A, B));
       }
-      __syncthreads();
+      GN_FENCE();
     }
-  }
+  });
 }
 
-// dw, db: the workgroups' rows summed column by column, in a fixed order: 16 columns x 64 row lanes
+// dw, db: the workgroups' rows summed column by column, in a fixed order (8 columns x 128 row lanes a workgroup); the workgroups behind those
+// combine the partial sums of long segments
 __global__ void __launch_bounds__(1024)
-k_gn_wsum(const float* __restrict__ part, int rows, int C, void* dw, void* db, int dt) {
-  __shared__ float red[64][17];
-  const int col = blockIdx.x * 16 + (threadIdx.x & 15), lane = threadIdx.x >> 4;
+k_gn_wsum(const DgGn a, int rows, int wblocks, void* dw, void* db, int dt) {
+  __shared__ float red[128][9];
+  if ((int)blockIdx.x >= wblocks) {
+    gn_join<true>(a, (int64_t)(blockIdx.x - wblocks) * 64 + (threadIdx.x >> 4));
+    return;
+  }
+  const int c = threadIdx.x & 7, col = blockIdx.x * 8 + c, lane = threadIdx.x >> 3;
   float s = 0.f;
-  if (col < 2 * C)
-    for (int r = lane; r < rows; r += 64) s += part[(int64_t)r * 2 * C + col];
-  red[lane][threadIdx.x & 15] = s;
+  if (col < 2 * a.C) {
+    const float* const p = a.wpart + col;
+#pragma unroll 8
+    for (int r = lane; r < rows; r += 128) s += p[(int64_t)r * 2 * a.C];
+  }
+  red[lane][c] = s;
   __syncthreads();
-  for (int o = 32; o; o >>= 1) {
-    if (lane < o) red[lane][threadIdx.x & 15] += red[lane + o][threadIdx.x & 15];
+  for (int o = 64; o; o >>= 1) {
+    if (lane < o) red[lane][c] += red[lane + o][c];
     __syncthreads();
   }
-  if (lane == 0 && col < 2 * C) {
-    void* const out = col < C ? dw : db;
-    if (out) dg_store_as(out, col < C ? col : col - C, dt, red[0][threadIdx.x & 15]);
+  if (lane == 0 && col < 2 * a.C) {
+    void* const out = col < a.C ? dw : db;
+    if (out) dg_store_as(out, col < a.C ? col : col - a.C, dt, red[0][c]);
   }
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------------------
-// vectors a thread holds: 8 of x, or 4 of x and dy (32 registers); twice as many where a vector is one register or half of one
-static constexpr int gn_nv(int vec_bytes, bool bwd) { return (bwd ? 4 : 8) * (vec_bytes <= 4 ? 2 : 1); }
+// vectors a thread holds: 8 of x (of up to 16 bytes) forward, 16 where they are one register or half of one; 8 of x and dy (of up to 8 bytes) backward
+static constexpr int gn_nv(int vec_bytes, bool bwd) { return bwd ? 8 : vec_bytes <= 4 ? 16 : 8; }
 
 // everything that follows from the shape; false: the shape is outside what this build handles
 static bool gn_plan(DgGn* a, int dtype, int vec_cap, bool bwd, int* vec, int* threads, int* tiles) {
-  const int full = dtype == DGCNN_F32 ? 4 : 8;
+  // (backward: 8-byte vectors.  16-byte ones take 171 registers with w, b and the sums of dw and db, two waves a SIMD: 115 us against 49 for the
+  // first launch of 2048 graphs of 128 bf16 channels)
+  const int full = (dtype == DGCNN_F32 ? 4 : 8) >> bwd;
   int v = full < vec_cap ? full : vec_cap;
   while (a->D % v) v >>= 1;
   a->DV = a->D / v;
   const int most = gn_most(v);
-  if (a->DV > most) return false;
+  if (a->DV > most || a->D > GN_MAX_D) return false;
   const int nv = gn_nv(v * dg_dtype_size(dtype), bwd), cols = a->DV * a->G;
   int t = GN_T;
   while (t < most && (a->DV > t || cols > t)) t *= 2;      // one column tile if the threads suffice
   a->Gt = cols <= t ? a->G : t / a->DV;
+  // (512 threads, or fewer groups a workgroup, hold segments twice as long: fewer of them are split, but fewer workgroups are resident.  2048 graphs of 74
+  // rows on average, 128 bf16 channels: backward 79 us as it is, 89 with half the groups, 160 with both; forward 44, 43, 43)
   a->CVt = a->Gt * a->DV;
-  // a wider workgroup where that lets it hold segments of up to twice the average length (they differ); where none could, many small chunks
-  const int64_t want = a->B ? 2 * ((a->N + a->B - 1) / a->B) : 0;
-  if ((int64_t)(most / a->CVt) * nv >= want)
-    while (t < most && (int64_t)(t / a->CVt) * nv < want) t *= 2;
   a->RY = t / a->CVt;
   a->R = a->RY * nv;
-  a->P = 64;
-  while (a->P > 1 && a->P * a->Gt > t) a->P >>= 1;
+  const int items = a->RY * a->DV;
+  a->P = items <= 64 ? 4 : items <= 512 ? 16 : 64;
+  while (a->P > 1 && a->P * a->Gt > t) a->P >>= 2;
   *vec = v; *threads = t; *tiles = (a->G + a->Gt - 1) / a->Gt;
   return true;
 }
 // which workgroups run: see the head of the file
 static void gn_grid(DgGn* a, int es, bool bwd) {
-  const bool one_long = a->ptr ? a->N > a->R : a->per > a->R;      // can any segment be longer than a chunk?
-  const bool all_long = !a->ptr && a->per > a->R;                  // are all?
-  // A long segment is worth a second launch (2 us) from 256 KB on: one workgroup streams ~100 bytes a nanosecond.
-  a->relaxed = one_long && a->N * a->C * es <= 256 * 1024;
-  const bool split = one_long && !a->relaxed;
-  a->nseg = all_long && split ? 0 : bwd && a->B > GN_WROWS ? GN_WROWS : a->B;
-  a->nchunk = split ? (int)((a->N + a->R - 1) / a->R) : 0;
-  a->cgrid = a->nchunk < GN_WROWS ? a->nchunk : GN_WROWS;
+  // Up to 512 KB in all no split is worth its two more launches (4 us each): any segment then passes through its workgroup (STREAM), read again
+  // for each sum out of the caches.
+  a->L = a->N * a->C * es <= 512 * 1024 && (a->ptr ? a->N : a->per) > a->R ? a->N : a->R;
+  const bool one_long = (a->ptr ? a->N : a->per) > a->L;      // can any segment be longer?
+  a->nseg = one_long && !a->ptr ? 0 : bwd && a->B > GN_WROWS ? GN_WROWS : a->B;      // (dense samples: all or none)
+  a->nchunk = one_long ? (int)((a->N + a->R - 1) / a->R) : 0;
+  const int most = bwd ? 1024 : 2048;      // (backward: a row of partial sums each)
+  a->cgrid = a->nchunk < most ? a->nchunk : most;
 }
 static bool gn_shape(DgGn* a, int64_t rows, int C, int groups, int segments) {
   if (rows < 0 || C < 1 || groups < 1 || C % groups || segments < 0) return false;
   a->N = rows; a->B = segments; a->C = C; a->G = groups; a->D = C / groups;
   return true;
 }
-static int64_t gn_part_bytes(const DgGn& a) { return dg_align(((int64_t)a.nchunk + a.B) * a.G * 2 * 4, 256); }
+static int64_t gn_part_bytes(const DgGn& a) { return a.nchunk ? dg_align(((int64_t)a.nchunk + a.B) * a.G * 2 * 4, 256) : 0; }
+static int64_t gn_ac_bytes(const DgGn& a) { return a.nchunk ? dg_align((int64_t)a.B * a.G * 2 * 4, 256) : 0; }
 
 // the plan of a call; alignment of the tensors (a multiple of the vector's bytes) is known at the call only, so the workspace is for the worst
 extern "C" int64_t dgcnn_group_norm_workspace_bytes(int64_t rows, int C, int groups, int segments, int dense, int dtype, int backward) {
@@ -591,21 +700,29 @@ extern "C" int64_t dgcnn_group_norm_workspace_bytes(int64_t rows, int C, int gro
     a.per = dense ? rows / segments : 0;
     if (!gn_plan(&a, dtype, cap, backward != 0, &v, &t, &n)) continue;
     gn_grid(&a, dg_dtype_size(dtype), backward != 0);
-    const int64_t b = (a.nchunk ? gn_part_bytes(a) : 0) + (backward ? dg_align(((int64_t)a.nseg + a.cgrid) * 2 * C * 4, 256) : 0);
+    const int64_t b = gn_part_bytes(a) + (backward ? gn_ac_bytes(a) + dg_align(((int64_t)a.nseg + a.cgrid) * 2 * C * 4, 256) : 0);
     if (b > most) most = b;
   }
   return most;
 }
 
 typedef void (*gn_kernel)(const DgGn);
+enum { GN_FWD, GN_FWD_STREAM, GN_FWD_LONG, GN_BWD, GN_BWD_STREAM, GN_BWD_LONG };
 template <class D, int VEC> static gn_kernel gn_pick(int which) {
   constexpr int F = gn_nv(VEC * sizeof(typename D::S), false), W = gn_nv(VEC * sizeof(typename D::S), true);
   switch (which) {
-    case 0: return (gn_kernel)k_gn_fwd<D, VEC, F>;
-    case 1: return (gn_kernel)k_gn_fwd_long<D, VEC, F>;
-    case 2: return (gn_kernel)k_gn_bwd<D, VEC, W>;
-    default: return (gn_kernel)k_gn_bwd_long<D, VEC, W>;
+    case GN_FWD: return (gn_kernel)k_gn_fwd<D, VEC, F, false>;
+    case GN_FWD_STREAM: return (gn_kernel)k_gn_fwd<D, VEC, F, true>;
+    case GN_FWD_LONG: return (gn_kernel)k_gn_fwd_long<D, VEC, F>;
   }
+  if constexpr (VEC < D::FULL) {      // (backward: vectors of up to 8 bytes)
+    switch (which) {
+      case GN_BWD: return (gn_kernel)k_gn_bwd<D, VEC, W, false>;
+      case GN_BWD_STREAM: return (gn_kernel)k_gn_bwd<D, VEC, W, true>;
+      case GN_BWD_LONG: return (gn_kernel)k_gn_bwd_long<D, VEC, W>;
+    }
+  }
+  return nullptr;
 }
 template <class D> static gn_kernel gn_pick_vec(int vec, int which) {
   if constexpr (D::FULL == 8) { if (vec == 8) return gn_pick<D, 8>(which); }
@@ -646,10 +763,12 @@ extern "C" int dgcnn_group_norm_fwd(const dgcnn_group_norm_args* p, void* y, voi
   if (!gn_plan(&a, p->dtype, cap, false, &vec, &threads, &tiles)) return DGCNN_EUNSUPPORTED;
   gn_grid(&a, dg_dtype_size(p->dtype), false);
   a.part = static_cast<float*>(ws);
-  hipLaunchKernelGGL(gn_pick_dtype(p->dtype, vec, 0), dim3(a.nseg + a.cgrid, tiles), dim3(threads), 0, (hipStream_t)stream, a);
+  hipLaunchKernelGGL(gn_pick_dtype(p->dtype, vec, a.L > a.R ? GN_FWD_STREAM : GN_FWD), dim3(a.nseg + a.cgrid, tiles), dim3(threads), 0, (hipStream_t)stream, a);
   DG_CHECK_LAUNCH();
   if (a.cgrid) {
-    hipLaunchKernelGGL(gn_pick_dtype(p->dtype, vec, 1), dim3(a.nchunk, tiles), dim3(threads), 0, (hipStream_t)stream, a);
+    hipLaunchKernelGGL(k_gn_join, dim3((unsigned)(((int64_t)a.B * a.G + 15) / 16)), dim3(256), 0, (hipStream_t)stream, a);
+    DG_CHECK_LAUNCH();
+    hipLaunchKernelGGL(gn_pick_dtype(p->dtype, vec, GN_FWD_LONG), dim3(a.nchunk, tiles), dim3(threads), 0, (hipStream_t)stream, a);
     DG_CHECK_LAUNCH();
   }
   return DGCNN_OK;
@@ -664,7 +783,7 @@ extern "C" int dgcnn_group_norm_bwd(const dgcnn_group_norm_args* p, const void* 
   if (!none && (!dy || !dx || !ws)) return DGCNN_EINVAL;
   if (none) {      // (empty sums; dx has no row that lies in a segment)
     if (dweight || dbias) {
-      hipLaunchKernelGGL(k_gn_wsum, dim3(dg_cdiv(2 * a.C, 16)), dim3(1024), 0, (hipStream_t)stream, (const float*)nullptr, 0, a.C, dweight, dbias, p->weight_dtype);
+      hipLaunchKernelGGL(k_gn_wsum, dim3(dg_cdiv(2 * a.C, 8)), dim3(1024), 0, (hipStream_t)stream, a, 0, dg_cdiv(2 * a.C, 8), dweight, dbias, p->weight_dtype);
       DG_CHECK_LAUNCH();
     }
     return DGCNN_OK;
@@ -675,15 +794,19 @@ extern "C" int dgcnn_group_norm_bwd(const dgcnn_group_norm_args* p, const void* 
   if (!gn_plan(&a, p->dtype, cap, true, &vec, &threads, &tiles)) return DGCNN_EUNSUPPORTED;
   gn_grid(&a, dg_dtype_size(p->dtype), true);
   a.part = static_cast<float*>(ws);
-  if (dweight || dbias) a.wpart = reinterpret_cast<float*>(static_cast<char*>(ws) + (a.nchunk ? gn_part_bytes(a) : 0));
-  hipLaunchKernelGGL(gn_pick_dtype(p->dtype, vec, 2), dim3(a.nseg + a.cgrid, tiles), dim3(threads), 0, (hipStream_t)stream, a);
+  char* const after = static_cast<char*>(ws) + gn_part_bytes(a);
+  a.ac = reinterpret_cast<float*>(after);
+  if (dweight || dbias) a.wpart = reinterpret_cast<float*>(after + gn_ac_bytes(a));
+  hipLaunchKernelGGL(gn_pick_dtype(p->dtype, vec, a.L > a.R ? GN_BWD_STREAM : GN_BWD), dim3(a.nseg + a.cgrid, tiles), dim3(threads), 0, (hipStream_t)stream, a);
   DG_CHECK_LAUNCH();
-  if (a.cgrid) {
-    hipLaunchKernelGGL(gn_pick_dtype(p->dtype, vec, 3), dim3(a.nchunk, tiles), dim3(threads), 0, (hipStream_t)stream, a);
+  const int wblocks = a.wpart ? dg_cdiv(2 * a.C, 8) : 0;
+  const int64_t jblocks = a.cgrid ? ((int64_t)a.B * a.G + 63) / 64 : 0;
+  if (wblocks + jblocks) {
+    hipLaunchKernelGGL(k_gn_wsum, dim3((unsigned)(wblocks + jblocks)), dim3(1024), 0, (hipStream_t)stream, a, a.nseg + a.cgrid, wblocks, dweight, dbias, p->weight_dtype);
     DG_CHECK_LAUNCH();
   }
-  if (a.wpart) {
-    hipLaunchKernelGGL(k_gn_wsum, dim3(dg_cdiv(2 * a.C, 16)), dim3(1024), 0, (hipStream_t)stream, (const float*)a.wpart, a.nseg + a.cgrid, a.C, dweight, dbias, p->weight_dtype);
+  if (a.cgrid) {
+    hipLaunchKernelGGL(gn_pick_dtype(p->dtype, vec, GN_BWD_LONG), dim3(a.nchunk, tiles), dim3(threads), 0, (hipStream_t)stream, a);
     DG_CHECK_LAUNCH();
   }
   return DGCNN_OK;
