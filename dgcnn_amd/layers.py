@@ -11,7 +11,6 @@ package there is no CPU fallback: CPU tensors raise :class:`dgcnn_amd._lib.Dgcnn
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 from typing import Optional
 
@@ -25,33 +24,57 @@ _DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _l
 ACTS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "tanh": 4}
 
 
-def _refuse(cond: bool, msg: str) -> None:
-    if cond:
-        raise _lib.DgcnnError(msg)
+def _no(msg: str):
+    raise _lib.DgcnnError(msg)
 
 
-def _dtype(t: torch.Tensor, what: str) -> int:
-    d = _DTYPES.get(t.dtype)
-    _refuse(d is None, f"{what} must be float32, bfloat16 or float16, got {t.dtype}")
-    return d
+def _no_type(t: torch.Tensor, what: str):
+    _no(f"{what} must be float32, bfloat16 or float16, got {t.dtype}")
 
 
-def _on(device: torch.device):
-    """The device a launch goes to has to be the current one."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
+def _no_gpu():
+    _no("dgcnn_amd.layers runs only on an AMD GPU through libdgcnn_hip.so; got a CPU tensor (there is deliberately no CPU fallback)")
 
 
-def _stream(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+def _launch(fn, name: str, device: torch.device, *args) -> None:
+    """One call of the library on the current stream of `device`, which has to be the current device for it."""
+    index = device.index
+    if index is None or index == torch.cuda.current_device():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        _lib.check(rc, name)
+
+
+_BYTES = {}      # workspace sizes: pure functions of their arguments (one library call a step otherwise)
+
+
+def _bytes(name: str, *args) -> int:
+    key = (name, *args)
+    n = _BYTES.get(key)
+    if n is None:
+        if len(_BYTES) > 4096:
+            _BYTES.clear()
+        n = _BYTES[key] = _lib.checked_bytes(getattr(_lib.lib(), name)(*args), name)
+    return n
 
 
 def _check_ptr(ptr: torch.Tensor, x: torch.Tensor) -> torch.Tensor:
-    _refuse(ptr.dim() != 1 or ptr.numel() < 1, f"ptr must be [segments + 1], got {tuple(ptr.shape)}")
-    _refuse(ptr.dtype not in (torch.int64, torch.int32), f"ptr must be int64 or int32, got {ptr.dtype}")
-    _refuse(ptr.device != x.device, f"ptr on {ptr.device}, x on {x.device}")
+    if ptr.dim() != 1 or ptr.numel() < 1:
+        _no(f"ptr must be [segments + 1], got {tuple(ptr.shape)}")
+    if ptr.dtype is not torch.int64 and ptr.dtype is not torch.int32:
+        _no(f"ptr must be int64 or int32, got {ptr.dtype}")
+    if ptr.get_device() != x.get_device():
+        _no(f"ptr on {ptr.device}, x on {x.device}")
+    if ptr.dtype is torch.int64 and ptr.is_contiguous():
+        return ptr
     return ptr.to(torch.int64).contiguous()
+
+
+def _wants_grad(*ts) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
 
 
 def graph_ptr(data) -> torch.Tensor:
@@ -65,47 +88,43 @@ def graph_ptr(data) -> torch.Tensor:
 
 
 # ---- products grouped by type ----------------------------------------------------------------------------------------------------------
+def _grouped_args(x, weight, bias, ptr):
+    rows, fin = x.shape
+    groups, fout = weight.shape[:2]
+    return _lib.GroupedLinearArgs(rows, max(x.stride(0), fin), fin, fout, groups, _DTYPES[x.dtype], x.data_ptr(), weight.data_ptr(),
+                                  None if bias is None else bias.data_ptr(), ptr.data_ptr())
+
+
+def _grouped_forward(x, weight, bias, ptr):
+    a = _grouped_args(x, weight, bias, ptr)
+    y = x.new_empty(a.rows, a.out_features)
+    _launch(_lib.lib().dgcnn_grouped_linear_fwd, "dgcnn_grouped_linear_fwd", x.device, ctypes.byref(a), y.data_ptr())
+    return y
+
+
 class _GroupedLinear(torch.autograd.Function):
     @staticmethod
-    def _args(x, weight, bias, ptr):
-        a = _lib.GroupedLinearArgs()
-        a.rows, a.in_features = x.shape
-        a.groups, a.out_features = weight.shape[:2]
-        a.ldx, a.dtype = max(x.stride(0), a.in_features), _DTYPES[x.dtype]
-        a.x, a.weight, a.ptr = x.data_ptr(), weight.data_ptr(), ptr.data_ptr()
-        a.bias = None if bias is None else bias.data_ptr()
-        return a
-
-    @staticmethod
     def forward(ctx, x, weight, bias, ptr):
-        if x.stride(1) != 1 or (x.shape[0] > 1 and x.stride(0) < x.shape[1]):
-            x = x.contiguous()
-        weight = weight.contiguous()
-        bias = None if bias is None else bias.contiguous()
-        a = _GroupedLinear._args(x, weight, bias, ptr)
-        y = torch.empty(a.rows, a.out_features, dtype=x.dtype, device=x.device)
-        with _on(x.device):
-            _lib.check(_lib.lib().dgcnn_grouped_linear_fwd(ctypes.byref(a), y.data_ptr(), _stream(x.device)), "dgcnn_grouped_linear_fwd")
         ctx.save_for_backward(x, weight, bias, ptr)
-        return y
+        return _grouped_forward(x, weight, bias, ptr)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
         x, weight, bias, ptr = ctx.saved_tensors
-        a = _GroupedLinear._args(x, weight, bias, ptr)
-        dy = dy.contiguous()
+        a = _grouped_args(x, weight, bias, ptr)
+        if not dy.is_contiguous():
+            dy = dy.contiguous()
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        dx = torch.empty(a.rows, a.in_features, dtype=x.dtype, device=x.device) if need_x else None
+        dx = x.new_empty(a.rows, a.in_features) if need_x else None
         dw = torch.empty_like(weight) if need_w or need_b else None
         db = torch.empty_like(bias) if need_b else None
-        L, ws = _lib.lib(), None
+        ws = None
         if dw is not None:
-            ws = torch.empty(_lib.checked_bytes(L.dgcnn_grouped_linear_workspace_bytes(a.rows, a.in_features, a.out_features, a.groups, a.dtype),
-                                                "dgcnn_grouped_linear_workspace_bytes"), dtype=torch.uint8, device=x.device)
-        at = lambda t: None if t is None else t.data_ptr()      # noqa: E731
-        with _on(x.device):
-            _lib.check(L.dgcnn_grouped_linear_bwd(ctypes.byref(a), dy.data_ptr(), at(dx), at(dw), at(db), at(ws), _stream(x.device)), "dgcnn_grouped_linear_bwd")
+            ws = torch.empty(_bytes("dgcnn_grouped_linear_workspace_bytes", a.rows, a.in_features, a.out_features, a.groups, a.dtype), dtype=torch.uint8,
+                             device=x.device)
+        _launch(_lib.lib().dgcnn_grouped_linear_bwd, "dgcnn_grouped_linear_bwd", x.device, ctypes.byref(a), dy.data_ptr(), None if dx is None else dx.data_ptr(),
+                None if dw is None else dw.data_ptr(), None if db is None else db.data_ptr(), None if ws is None else ws.data_ptr())
         return dx, dw if need_w else None, db, None
 
 
@@ -115,16 +134,25 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, ptr: torch.Tensor, bia
 
     Groups may be empty; rows outside every group give 0 and get gradient 0.  Everything of one type; sums in fp32, results rounded once.  The rows
     of ``x`` may be strided.  Differentiable once in ``x``, ``weight`` and ``bias``."""
-    _refuse(not x.is_cuda, "dgcnn_amd.layers runs only on an AMD GPU through libdgcnn_hip.so; got a CPU tensor (there is deliberately no CPU fallback)")
-    _refuse(x.dim() != 2 or weight.dim() != 3 or x.shape[1] != weight.shape[2] or min(weight.shape[1:]) < 1,
-            f"x must be [N, in] and weight [groups, out, in], got {tuple(x.shape)} and {tuple(weight.shape)}")
-    _dtype(x, "x")
-    _refuse(weight.dtype != x.dtype or weight.device != x.device, f"weight must be {x.dtype} on {x.device}, got {weight.dtype} on {weight.device}")
-    if bias is not None:
-        _refuse(bias.shape != weight.shape[:2] or bias.dtype != x.dtype or bias.device != x.device,
-                f"bias must be {tuple(weight.shape[:2])} {x.dtype} on {x.device}, got {tuple(bias.shape)} {bias.dtype} on {bias.device}")
+    if not x.is_cuda:
+        _no_gpu()
+    if x.dim() != 2 or weight.dim() != 3 or x.shape[1] != weight.shape[2] or min(weight.shape[1:]) < 1:
+        _no(f"x must be [N, in] and weight [groups, out, in], got {tuple(x.shape)} and {tuple(weight.shape)}")
+    if x.dtype not in _DTYPES:
+        _no_type(x, "x")
+    if weight.dtype != x.dtype or weight.get_device() != x.get_device():
+        _no(f"weight must be {x.dtype} on {x.device}, got {weight.dtype} on {weight.device}")
+    if bias is not None and (bias.shape != weight.shape[:2] or bias.dtype != x.dtype or bias.get_device() != x.get_device()):
+        _no(f"bias must be {tuple(weight.shape[:2])} {x.dtype} on {x.device}, got {tuple(bias.shape)} {bias.dtype} on {bias.device}")
     ptr = _check_ptr(ptr, x)
-    _refuse(ptr.numel() != weight.shape[0] + 1, f"ptr must be [{weight.shape[0] + 1}] for {weight.shape[0]} groups, got [{ptr.numel()}]")
+    if ptr.numel() != weight.shape[0] + 1:
+        _no(f"ptr must be [{weight.shape[0] + 1}] for {weight.shape[0]} groups, got [{ptr.numel()}]")
+    if x.stride(1) != 1 or (x.shape[0] > 1 and x.stride(0) < x.shape[1]):      # (rows may be strided; anything else is copied)
+        x = x.contiguous()
+    weight = weight.contiguous()
+    bias = None if bias is None else bias.contiguous()
+    if not _wants_grad(x, weight, bias):
+        return _grouped_forward(x, weight, bias, ptr)
     return _GroupedLinear.apply(x, weight, bias, ptr)
 
 
@@ -148,51 +176,44 @@ class GroupedLinear(nn.Module):
 
 
 # ---- group norm ----------------------------------------------------------------------------------------------------------------------
+def _norm_forward(x, weight, bias, ptr, groups, eps, act):
+    C = x.shape[-1]
+    segments = x.shape[0] if ptr is None else ptr.numel() - 1
+    rows = x.numel() // C
+    some = weight if weight is not None else bias
+    dtype = _DTYPES[x.dtype]
+    y = torch.empty_like(x) if segments else torch.zeros_like(x)
+    stats = torch.empty(2, segments, groups, dtype=torch.float32, device=x.device)
+    ws = torch.empty(_bytes("dgcnn_group_norm_workspace_bytes", rows, C, groups, segments, ptr is None, dtype, 0), dtype=torch.uint8, device=x.device)
+    at = stats.data_ptr()
+    args = (rows, C, groups, segments, dtype, 0 if some is None else _DTYPES[some.dtype], act, eps, 0, x.data_ptr(),
+            None if weight is None else weight.data_ptr(), None if bias is None else bias.data_ptr(), None if ptr is None else ptr.data_ptr(),
+            at, at + 4 * segments * groups)
+    _launch(_lib.lib().dgcnn_group_norm_fwd, "dgcnn_group_norm_fwd", x.device, ctypes.byref(_lib.GroupNormArgs(*args)), y.data_ptr(), ws.data_ptr())
+    return y, stats, args
+
+
 class _GroupNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, ptr, groups, eps, act):
-        C = x.shape[-1]
-        xc = x.contiguous()
-        segments = x.shape[0] if ptr is None else ptr.numel() - 1
-        rows = xc.numel() // C
-        a = _lib.GroupNormArgs()
-        a.rows, a.channels, a.groups, a.segments, a.dtype, a.act, a.eps = rows, C, groups, segments, _DTYPES[x.dtype], act, eps
-        wb = [None if t is None else t.contiguous() for t in (weight, bias)]
-        some = wb[0] if wb[0] is not None else wb[1]
-        a.weight_dtype = 0 if some is None else _DTYPES[some.dtype]
-        y = torch.empty_like(xc) if segments else torch.zeros_like(xc)
-        stats = torch.empty(2, segments, groups, dtype=torch.float32, device=x.device)
-        L = _lib.lib()
-        ws = torch.empty(_lib.checked_bytes(L.dgcnn_group_norm_workspace_bytes(rows, C, groups, segments, ptr is None, a.dtype, 0),
-                                            "dgcnn_group_norm_workspace_bytes"), dtype=torch.uint8, device=x.device)
-        a.x, a.mean, a.rstd = xc.data_ptr(), stats[0].data_ptr(), stats[1].data_ptr()
-        a.weight, a.bias = (None if t is None else t.data_ptr() for t in wb)
-        a.ptr = None if ptr is None else ptr.data_ptr()
-        with _on(x.device):
-            _lib.check(L.dgcnn_group_norm_fwd(ctypes.byref(a), y.data_ptr(), ws.data_ptr(), _stream(x.device)), "dgcnn_group_norm_fwd")
-        ctx.save_for_backward(xc, *wb, ptr, stats)
-        ctx.args = (rows, C, groups, segments, a.dtype, a.weight_dtype, act, eps)
+        y, stats, ctx.args = _norm_forward(x, weight, bias, ptr, groups, eps, act)
+        ctx.save_for_backward(x, weight, bias, ptr, stats)      # (args hold the addresses of these)
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
         x, weight, bias, ptr, stats = ctx.saved_tensors
-        a = _lib.GroupNormArgs()
-        a.rows, a.channels, a.groups, a.segments, a.dtype, a.weight_dtype, a.act, a.eps = ctx.args
-        dyc = dy.contiguous()
-        dx = torch.empty_like(x) if a.segments else torch.zeros_like(x)
+        args = ctx.args
+        rows, C, groups, segments, dtype = args[:5]
+        if not dy.is_contiguous():
+            dy = dy.contiguous()
+        dx = torch.empty_like(x) if segments else torch.zeros_like(x)
         dw = torch.empty_like(weight) if ctx.needs_input_grad[1] else None
         db = torch.empty_like(bias) if ctx.needs_input_grad[2] else None
-        L = _lib.lib()
-        ws = torch.empty(_lib.checked_bytes(L.dgcnn_group_norm_workspace_bytes(a.rows, a.channels, a.groups, a.segments, ptr is None, a.dtype, 1),
-                                            "dgcnn_group_norm_workspace_bytes"), dtype=torch.uint8, device=x.device)
-        a.x, a.mean, a.rstd = x.data_ptr(), stats[0].data_ptr(), stats[1].data_ptr()
-        a.weight, a.bias = (None if t is None else t.data_ptr() for t in (weight, bias))
-        a.ptr = None if ptr is None else ptr.data_ptr()
-        with _on(x.device):
-            _lib.check(L.dgcnn_group_norm_bwd(ctypes.byref(a), dyc.data_ptr(), dx.data_ptr(), None if dw is None else dw.data_ptr(),
-                                              None if db is None else db.data_ptr(), ws.data_ptr(), _stream(x.device)), "dgcnn_group_norm_bwd")
+        ws = torch.empty(_bytes("dgcnn_group_norm_workspace_bytes", rows, C, groups, segments, ptr is None, dtype, 1), dtype=torch.uint8, device=x.device)
+        _launch(_lib.lib().dgcnn_group_norm_bwd, "dgcnn_group_norm_bwd", x.device, ctypes.byref(_lib.GroupNormArgs(*args)), dy.data_ptr(), dx.data_ptr(),
+                None if dw is None else dw.data_ptr(), None if db is None else db.data_ptr(), ws.data_ptr())
         return dx, dw, db, None, None, None, None
 
 
@@ -205,22 +226,36 @@ def group_norm(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tensor] 
     ``ptr[s] .. ptr[s + 1] - 1`` (ascending, on the device; never read by the host); samples may be empty, rows outside every sample give 0 and
     get gradient 0.  ``act``: "none", "relu", "silu", "gelu" (with erf) or "tanh".  ``weight`` and ``bias`` may be of another type than ``x``;
     ``y`` is of ``x``'s.  Differentiable once in ``x``, ``weight`` and ``bias``."""
-    _refuse(act not in ACTS, f"act must be one of {sorted(ACTS)}, got {act!r}")
-    _refuse(not x.is_cuda, "dgcnn_amd.layers runs only on an AMD GPU through libdgcnn_hip.so; got a CPU tensor (there is deliberately no CPU fallback)")
-    _refuse(x.dim() < 2, f"x must be [B, ..., C] or [N, C], got {tuple(x.shape)}")
-    _dtype(x, "x")
+    if act not in ACTS:
+        _no(f"act must be one of {sorted(ACTS)}, got {act!r}")
+    if not x.is_cuda:
+        _no_gpu()
+    if x.dim() < 2:
+        _no(f"x must be [B, ..., C] or [N, C], got {tuple(x.shape)}")
+    if x.dtype not in _DTYPES:
+        _no_type(x, "x")
     C = x.shape[-1]
-    _refuse(C < 1 or num_groups < 1 or C % num_groups != 0, f"num_groups {num_groups} does not divide {C} channels")
-    _refuse(not eps >= 0.0, f"eps must not be negative, got {eps}")
-    for name, t in (("weight", weight), ("bias", bias)):
+    if C < 1 or num_groups < 1 or C % num_groups != 0:
+        _no(f"num_groups {num_groups} does not divide {C} channels")
+    if not eps >= 0.0:
+        _no(f"eps must not be negative, got {eps}")
+    for t in (weight, bias):
         if t is not None:
-            _dtype(t, name)
-            _refuse(tuple(t.shape) != (C,) or t.device != x.device, f"{name} must be [{C}] on {x.device}, got {tuple(t.shape)} on {t.device}")
-    _refuse(weight is not None and bias is not None and weight.dtype != bias.dtype, "weight and bias must be of one type")
+            if t.dtype not in _DTYPES:
+                _no_type(t, "weight and bias")
+            if t.dim() != 1 or t.shape[0] != C or t.get_device() != x.get_device():
+                _no(f"weight and bias must be [{C}] on {x.device}, got {tuple(t.shape)} on {t.device}")
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        _no("weight and bias must be of one type")
     if ptr is not None:
-        _refuse(x.dim() != 2, f"with ptr, x must be [N, C], got {tuple(x.shape)}")
+        if x.dim() != 2:
+            _no(f"with ptr, x must be [N, C], got {tuple(x.shape)}")
         ptr = _check_ptr(ptr, x)
-    return _GroupNorm.apply(x, weight, bias, ptr, int(num_groups), float(eps), ACTS[act])
+    x = x.contiguous()
+    weight, bias = (None if t is None else t.contiguous() for t in (weight, bias))
+    if not _wants_grad(x, weight, bias):
+        return _norm_forward(x, weight, bias, ptr, num_groups, eps, ACTS[act])[0]
+    return _GroupNorm.apply(x, weight, bias, ptr, num_groups, eps, ACTS[act])
 
 
 class GroupNorm(nn.Module):

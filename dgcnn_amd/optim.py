@@ -20,6 +20,8 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import operator
+from array import array
 from itertools import chain
 from typing import Optional, Sequence, Union
 
@@ -224,15 +226,21 @@ def _capturing() -> bool:
     return torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing()
 
 
-def _check_list(name, ts, params, dtypes, blocks=False) -> None:
-    _refuse(len(ts) != len(params), f"{name}: {len(ts)} tensors for {len(params)} parameters")
-    dev = params[0].device
-    for t, p in zip(ts, params):
-        n = -(-p.numel() // STATE_BLOCK) if blocks else p.numel()
-        if t.dtype not in dtypes or t.numel() != n or t.device != dev or not (t.is_contiguous() if blocks else t.stride() == p.stride()):
-            raise _lib.DgcnnError(f"{name}: a tensor is {tuple(t.shape)} {t.dtype} on {t.device} with strides {t.stride()}; its parameter is {tuple(p.shape)} "
-                                  f"{p.dtype} on {dev} with strides {p.stride()} (types here: {', '.join(map(str, dtypes))}"
-                                  + (f"; [ceil(numel / {STATE_BLOCK})] contiguous)" if blocks else "; the parameter's shape and strides)"))
+_numel, _is_contiguous, _get_device, _data_ptr = (getattr(torch.Tensor, k) for k in ("numel", "is_contiguous", "get_device", "data_ptr"))
+_get_dtype = operator.attrgetter("dtype")
+
+
+def _check_list(name, ts, params, numels, device, dtypes) -> torch.dtype:
+    """Every tensor of one of `dtypes`, as large and laid out as its parameter (or, for scales, `numels` contiguous elements); the type."""
+    # (a few C loops over the whole list; the tensors are looked at one by one only to say which it is)
+    kinds = set(map(_get_dtype, ts))
+    if len(ts) == len(numels) and len(kinds) == 1 and kinds <= dtypes and set(map(_get_device, ts)) == device and list(map(_numel, ts)) == numels and \
+            (all(map(_is_contiguous, ts)) and (params is None or all(map(_is_contiguous, params)))
+             or params is not None and all(t.stride() == p.stride() for t, p in zip(ts, params))):
+        return kinds.pop()
+    raise _lib.DgcnnError(f"{name} must be {len(numels)} tensors of one type ({', '.join(sorted(map(str, dtypes)))}) on one device, "
+                          + (f"contiguous with one element for each {STATE_BLOCK} of the parameter" if params is None else "with their parameters' sizes and strides")
+                          + f"; got {len(ts)}: " + ", ".join(f"{t.dtype} {tuple(t.shape)} {t.stride()} on {t.device}" for t in list(ts)[:4]))
 
 
 def _dense(p) -> bool:
@@ -260,29 +268,29 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
         return
     p0 = params[0]
     dev = p0.device
-    _refuse(not p0.is_cuda, "dgcnn_amd.optim.adamw_step runs only on an AMD GPU through libdgcnn_hip.so; got a CPU tensor")
-    _refuse(p0.dtype not in _DTYPES, f"parameters must be float32, bfloat16 or float16, got {p0.dtype}")
-    for p in params:
-        if p.dtype != p0.dtype or p.device != dev or not _dense(p):
-            raise _lib.DgcnnError(f"parameters must be dense tensors of one type on one device: got {p0.dtype} on {dev} and {p.dtype} on {p.device} "
-                                  f"{tuple(p.shape)} with strides {p.stride()}")
+    if not p0.is_cuda:
+        _refuse(True, "dgcnn_amd.optim.adamw_step runs only on an AMD GPU through libdgcnn_hip.so; got a CPU tensor")
+    numels, device = list(map(_numel, params)), {p0.get_device()}
+    kind = _check_list("params", params, params, numels, device, _DTYPES.keys())
+    if not all(map(_is_contiguous, params)) and not all(map(_dense, params)):
+        _refuse(True, "parameters must be dense tensors")
     bits = 32 if exp_avg_scales is None else 8
-    _refuse((exp_avg_scales is None) != (exp_avg_sq_scales is None), "8-bit moments need both exp_avg_scales and exp_avg_sq_scales")
-    _refuse(len(grads) != len(params), f"grads: {len(grads)} tensors for {len(params)} parameters")
-    g0 = grads[0].dtype
-    _check_list("grads", grads, params, (p0.dtype,) if g0 == p0.dtype else (torch.float32,))
-    state = (torch.float32,) if bits == 32 else (torch.float8_e4m3fn,)
-    _check_list("exp_avgs", exp_avgs, params, state)
-    _check_list("exp_avg_sqs", exp_avg_sqs, params, state)
-    lists = [params, grads, exp_avgs, exp_avg_sqs]
-    for name, ts in (("exp_avg_scales", exp_avg_scales), ("exp_avg_sq_scales", exp_avg_sq_scales)):
-        if ts is not None:
-            _check_list(name, ts, params, (torch.float32,), blocks=True)
+    if (exp_avg_scales is None) != (exp_avg_sq_scales is None):
+        _refuse(True, "8-bit moments need both exp_avg_scales and exp_avg_sq_scales")
+    gkind = _check_list("grads", grads, params, numels, device, {kind, torch.float32})
+    state = {torch.float32} if bits == 32 else {torch.float8_e4m3fn}
+    _check_list("exp_avgs", exp_avgs, params, numels, device, state)
+    _check_list("exp_avg_sqs", exp_avg_sqs, params, numels, device, state)
+    if bits == 8:
+        blocks = [-(-n // STATE_BLOCK) for n in numels]
+        _check_list("exp_avg_scales", exp_avg_scales, None, blocks, device, {torch.float32})
+        _check_list("exp_avg_sq_scales", exp_avg_sq_scales, None, blocks, device, {torch.float32})
     if masters is not None:
-        _refuse(p0.dtype == torch.float32, "masters are for bfloat16 and float16 parameters")
-        _check_list("masters", masters, params, (torch.float32,))
-    _refuse(not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0), f"betas must lie in [0, 1), got {betas}")
-    _refuse(not eps >= 0.0, f"eps must not be negative, got {eps}")
+        if kind == torch.float32:
+            _refuse(True, "masters are for bfloat16 and float16 parameters")
+        _check_list("masters", masters, params, numels, device, {torch.float32})
+    if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0 and eps >= 0.0):
+        _refuse(True, f"betas must lie in [0, 1) and eps must not be negative, got {betas}, {eps}")
 
     a = _lib.AdamwArgs()
     keep = None
@@ -294,22 +302,27 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
             _refuse(lr.dtype != torch.float32 or lr.numel() != 1 or lr.device != dev, f"lr must be a float or a float32 tensor of one element on {dev}")
             a.lr_dev, lr = lr.data_ptr(), 0.0
     else:
-        _refuse(step < 1, f"step counts from 1, got {step}")
-        _refuse(isinstance(lr, torch.Tensor), "lr may be a tensor only where step is one")
-        _refuse(_capturing(), "a captured step needs its counter on the device: step as an int64 tensor (AdamW: capturable=True)")
+        if step < 1:
+            _refuse(True, f"step counts from 1, got {step}")
+        if isinstance(lr, torch.Tensor):
+            _refuse(True, "lr may be a tensor only where step is one")
+        if _capturing():
+            _refuse(True, "a captured step needs its counter on the device: step as an int64 tensor (AdamW: capturable=True)")
         a.step = step
     a.lr, a.beta1, a.beta2, a.eps, a.weight_decay = lr, betas[0], betas[1], eps, weight_decay
-    a.seed, a.first_index = seed & 0xFFFFFFFFFFFFFFFF, 0
-    a.param_dtype, a.grad_dtype, a.state_bits, a.count = _DTYPES[p0.dtype], _DTYPES[g0], bits, len(params)
+    a.seed = seed & 0xFFFFFFFFFFFFFFFF
+    a.param_dtype, a.grad_dtype, a.state_bits, a.count = _DTYPES[kind], _DTYPES[gkind], bits, len(params)
     none = [0] * len(params)
-    at = lambda ts: none if ts is None else [t.data_ptr() for t in ts]      # noqa: E731
-    where = at(params)
-    _refuse(len(set(where)) < sum(1 for p in params if p.numel()), "a parameter is in the list twice")
-    columns = [where, at(grads), at(exp_avgs), at(exp_avg_sqs), at(exp_avg_scales), at(exp_avg_sq_scales), at(masters), [p.numel() for p in params]]
-    table = (ctypes.c_int64 * (8 * len(params)))(*chain.from_iterable(zip(*columns)))
-    a.tensors = ctypes.addressof(table)
+    at = lambda ts: none if ts is None else map(_data_ptr, ts)      # noqa: E731
+    where = list(map(_data_ptr, params))
+    if len(set(where)) < len(where) and len({w for w, n in zip(where, numels) if n}) < sum(1 for n in numels if n):
+        _refuse(True, "a parameter is in the list twice")
+    table = array("q", chain.from_iterable(zip(where, at(grads), at(exp_avgs), at(exp_avg_sqs), at(exp_avg_scales), at(exp_avg_sq_scales), at(masters), numels)))
+    a.tensors = table.buffer_info()[0]
+    # (the launch goes to the tensors' device, which has to be the current one)
     with contextlib.nullcontext() if dev.index is None or dev.index == torch.cuda.current_device() else torch.cuda.device(dev):
-        _lib.check(_lib.lib().dgcnn_adamw_step(ctypes.byref(a), torch.cuda.current_stream(dev).cuda_stream), "dgcnn_adamw_step")
+        rc = _lib.lib().dgcnn_adamw_step(ctypes.byref(a), torch._C._cuda_getCurrentRawStream(dev.index))
+    _lib.check(rc, "dgcnn_adamw_step")
 
 
 class AdamW(Optimizer):
