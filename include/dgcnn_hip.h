@@ -376,7 +376,8 @@ int dgcnn_adamw_step(const dgcnn_adamw_args* args, dgcnn_stream_t stream);
  * weight [groups, out_features, in_features], bias [groups, out_features] or NULL, y and dy [rows, out_features], dx [rows, in_features]
  * (contiguous), everything of dtype.  ptr [groups + 1] int64 (device, ascending); groups may be empty (dweight and dbias 0); rows outside
  * every group give 0 in y and dx.  (A ptr that does not ascend, or points outside [0, rows], gives unspecified values, never an access outside
- * the tensors.)  _bwd: dx, dweight, dbias may each be NULL (dbias only with dweight); ws of dgcnn_grouped_linear_workspace_bytes. */
+ * the tensors.)  ldx and out_features: at most 2^21.  _bwd: dx, dweight, dbias may each be NULL (dbias only with dweight); ws of
+ * dgcnn_grouped_linear_workspace_bytes. */
 typedef struct dgcnn_grouped_linear_args {
   int64_t rows, ldx;
   int32_t in_features, out_features, groups, dtype;
