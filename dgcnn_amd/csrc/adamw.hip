@@ -93,13 +93,15 @@ __device__ __forceinline__ uint32_t aw_hash(uint32_t h) {             // the 32-
   return h ^ (h >> 16);
 }
 
-// largest finite magnitude over the 32 lanes that hold one block of 256 elements
+// largest finite magnitude over the 32 lanes that hold one block of 256 elements (the maximum passes over NaN; infinities are looked for where it is one)
 __device__ __forceinline__ float aw_block_max(const float* x) {
   float a = 0.f;
 #pragma unroll
-  for (int i = 0; i < AW_EPT; ++i) {
-    const float f = fabsf(x[i]);
-    a = fmaxf(a, f <= 3.4028235e38f ? f : 0.f);
+  for (int i = 0; i < AW_EPT; ++i) a = fmaxf(a, fabsf(x[i]));
+  if (a > 3.4028235e38f) {
+    a = 0.f;
+#pragma unroll
+    for (int i = 0; i < AW_EPT; ++i) a = fmaxf(a, fabsf(x[i]) <= 3.4028235e38f ? fabsf(x[i]) : 0.f);
   }
 #pragma unroll
   for (int o = 16; o; o >>= 1) a = fmaxf(a, __shfl_xor(a, o));
@@ -187,7 +189,10 @@ k_adamw(const DgAdamwTable t, const DgAdamwScalars byval, const DgAdamwScalars* 
       m[i] = m[i] * s.b1 + g[i] * s.omb1;
       v[i] = v[i] * s.b2 + (g[i] * g[i]) * s.omb2;
       r[i] = sqrtf(v[i]);
-      p[i] = p[i] * s.decay - (m[i] / (r[i] * s.rbc2 + s.eps)) * s.ss;
+      const float den = r[i] * s.rbc2 + s.eps;
+      // (8 bits: bound by arithmetic, and v_rcp_f32's 1 ulp of an update is far below its parameter's rounding)
+      const float u = BITS == 32 ? m[i] / den : m[i] * __builtin_amdgcn_rcpf(den);
+      p[i] = p[i] * s.decay - u * s.ss;
     }
     if (MASTER) aw_store<DgF32>(master + at, n, wide, p);
     aw_store<P>(param + at, n, wide, p);

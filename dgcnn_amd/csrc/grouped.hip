@@ -167,6 +167,8 @@ template <class D> __device__ __forceinline__ f32x4 gl_mfma(const gl_u32x4& a, c
   }
 }
 
+__device__ __forceinline__ int gl_wave() { return __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)); }      // (scalar)
+
 // One operand's tile: W indices (i or j) x R r values, ROWB = 64 or 128 bytes of them
 //   T = false: memory and LDS [index][r]; chunk c of an index at place c ^ (index / (256 / ROWB)): 16 lanes read one chunk of 16 indices, which are then 16
 //              different 16-byte pieces of the 256 bytes that the banks are wide
@@ -191,7 +193,7 @@ template <class D, int W, bool T, int ROWB> struct GlTile {
   // Whole tiles: the lane's offsets from the tile's first element (indices behind the operand's last one read that one: they end in rows and columns of
   // C that are not stored), the same for every step.
   template <int G, int THREADS> static __device__ __forceinline__ void offsets(int64_t ld, int64_t left, uint32_t* off) {
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int wave = gl_wave(), lane = threadIdx.x & 63;
 #pragma unroll
     for (int k = 0; k < loads<G, THREADS>(); ++k) {
       const int u = (k * (THREADS / 64) + wave) * 64 + lane;      // unit of G bytes
@@ -204,7 +206,7 @@ template <class D, int W, bool T, int ROWB> struct GlTile {
     }
   }
   template <int G, int THREADS> static __device__ __forceinline__ void load(char* lds, const S* base, const uint32_t* off) {
-    const int wave = threadIdx.x >> 6;
+    const int wave = gl_wave();
     const char* const at = gl_uniform(reinterpret_cast<const char*>(base));
 #pragma unroll
     for (int k = 0; k < loads<G, THREADS>(); ++k) gl_to_lds<G>(at, off[k], lds + (k * (THREADS / 64) + wave) * 64 * G);
@@ -212,7 +214,7 @@ template <class D, int W, bool T, int ROWB> struct GlTile {
   // the tile at (w0, r0) of an operand with nw indices and r values up to rend, zeros behind them
   template <int G, int THREADS>
   static __device__ __forceinline__ void load_part(char* lds, const S* base, int64_t ld, int64_t w0, int64_t r0, int64_t nw, int64_t rend) {
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int wave = gl_wave(), lane = threadIdx.x & 63;
     if constexpr (G >= 4) {
 #pragma unroll 4
       for (int k = 0; k < loads<G, THREADS>(); ++k) {
@@ -279,7 +281,7 @@ k_gl(const DgGl a) {
   constexpr int R = TP::R;
   constexpr int STAGE = TP::BYTES + TQ::BYTES, LP = TP::template loads<G, THREADS>(), LQ = TQ::template loads<G, THREADS>();      // (loads of a wave and stage)
   DG_DYN_SMEM(char, smem);                                    // ST stages of P and Q
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, l = lane & 15, g = lane >> 4;
+  const int wave = gl_wave(), lane = threadIdx.x & 63, l = lane & 15, g = lane >> 4;
   const int wi = wave / WJ, wj = wave - wi * WJ;
 
   // ---- which tile: C's rows lo .. (fewer than nw_i) and columns j0 .., the sum over r0 .. rend - 1
@@ -289,7 +291,7 @@ k_gl(const DgGl a) {
   GlItems items;
   if (!GRAD) {
     // consecutive tiles (the columns of one run of rows first) on one XCD: workgroups go to the eight in turn
-    constexpr int SHIFT = BI == 32 ? 5 : BI == 64 ? 6 : BI == 128 ? 7 : 8;
+    constexpr int SHIFT = BI == 16 ? 4 : BI == 32 ? 5 : BI == 64 ? 6 : BI == 128 ? 7 : 8;
     static_assert(BI == 1 << SHIFT, "rows a tile");
     const unsigned tiles = (unsigned)gl_total(a, a.E + 2, SHIFT, items) * a.tj, share = (tiles + 7) >> 3, t = (blockIdx.x & 7) * share + (blockIdx.x >> 3);
     if ((blockIdx.x >> 3) >= share || t >= tiles) return;
@@ -308,7 +310,9 @@ k_gl(const DgGl a) {
     }
     q += (int64_t)e * a.qstride;
   } else {
-    const unsigned tile = blockIdx.x % (unsigned)(a.ti * a.tj), t = blockIdx.x / (unsigned)(a.ti * a.tj);
+    // the tiles of a slice (or group), which read the same rows, on one XCD
+    const unsigned per = a.ti * a.tj, on = blockIdx.x >> 3, tile = on % per, t = on / per * 8 + (blockIdx.x & 7);
+    if (t >= (a.split ? (unsigned)a.slots : (unsigned)a.E)) return;
     if (a.split) {
       gl_total(a, a.E, a.shift, items);
       if (!gl_find(a, a.E, a.shift, (int)t, items, e, lo, hi)) return;
@@ -334,6 +338,28 @@ k_gl(const DgGl a) {
   gl_u32x4 ones;
 #pragma unroll
   for (int i = 0; i < 4; ++i) ones[i] = gl_ones<D>();
+
+  const bool whole4 = G == 16 || ((reinterpret_cast<uintptr_t>(a.c) & (4 * sizeof(S) - 1)) == 0 && (a.nj & 3) == 0);      // every four columns are one access
+  float b[GRAD ? 1 : FJ][4];      // the bias of the lane's columns: asked for here, long before it is added
+  if constexpr (!GRAD) {
+#pragma unroll
+    for (int j = 0; j < FJ; ++j) {
+      const int col = j0 + (wj * FJ + j) * 16 + 4 * g;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) b[j][k] = 0.f;
+      if (a.bias && col < a.nj) {
+        const S* const bias = static_cast<const S*>(a.bias) + (int64_t)e * a.nj;
+        if (G == 16) {
+          const DgRaw<D, 4> v = dg_load<D, 4>(bias + col);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) b[j][k] = v.get(k);
+        } else {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) b[j][k] = D::to(bias[min(col + k, a.nj - 1)]);
+        }
+      }
+    }
+  }
 
   // ---- ST stages: ST - 1 of them are on their way or being multiplied, the one that was multiplied last is loaded anew.  One barrier a step: it
   // says that this step's stage has arrived (all but the ST - 2 newer ones' loads are done) and that everyone is through with the last one.
@@ -401,16 +427,9 @@ k_gl(const DgGl a) {
     return;
   }
   S* const c = static_cast<S*>(a.c) + (GRAD ? (int64_t)e * a.ni * a.nj : 0) + lo * a.ldc + j0;
-  const bool whole4 = G == 16 || ((reinterpret_cast<uintptr_t>(a.c) & (4 * sizeof(S) - 1)) == 0 && (a.nj & 3) == 0);      // every four columns are one store
 #pragma unroll
   for (int j = 0; j < FJ; ++j) {
     const int n = wide - (col + 16 * j);      // columns that are there
-    float b[4] = {0.f, 0.f, 0.f, 0.f};
-    if (!GRAD && a.bias) {
-      const S* const bias = static_cast<const S*>(a.bias) + (int64_t)e * a.nj + j0 + col + 16 * j;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) if (k < n) b[k] = D::to(bias[k]);
-    }
 #pragma unroll
     for (int i = 0; i < FI; ++i) {
       if (row + 16 * i >= left || n <= 0) continue;
@@ -418,11 +437,11 @@ k_gl(const DgGl a) {
       if (whole4) {
         DgRaw<D, 4> o;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) o.set(k, acc[i][j][k] + b[k]);
+        for (int k = 0; k < 4; ++k) o.set(k, GRAD ? acc[i][j][k] : acc[i][j][k] + b[GRAD ? 0 : j][k]);
         dg_store<D, 4>(at, o);
       } else {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) if (k < n) at[k] = D::from(acc[i][j][k] + b[k]);
+        for (int k = 0; k < 4; ++k) if (k < n) at[k] = D::from(GRAD ? acc[i][j][k] : acc[i][j][k] + b[GRAD ? 0 : j][k]);
       }
     }
   }
@@ -476,6 +495,9 @@ k_gl_join(const DgGl a) {
   }
 }
 
+#ifndef GL_FEW
+#define GL_FEW 16
+#endif
 // ---- host ------------------------------------------------------------------------------------------------------------------------
 typedef void (*gl_kernel)(const DgGl);
 struct GlForm { gl_kernel k; int bi, bj, threads, lds; };
@@ -486,15 +508,21 @@ template <class D, int WI, int WJ, int FI, int FJ, int ST, int ROWB, bool PT, bo
   f.lds = ST * (f.bi + f.bj) * ROWB;
   return f;
 }
-#ifndef GL_BIG
-#define GL_BIG 2, 2, 4, 4, 2, 128
-#endif
-template <class D, bool PT, bool QT> static GlForm gl_pick(int nj, bool aligned) {
+// A tile for the shape (rows: of the whole call; nj: columns of C)
+template <class D, bool PT, bool QT> static GlForm gl_pick(int64_t rows, int E, int nj, bool aligned) {
+  constexpr bool WIDE = sizeof(typename D::S) == 4;
+  if constexpr (!PT) {
+    if (rows <= GL_FEW * (int64_t)E) return gl_form<D, 1, 2, 1, 1, 6, 128, PT, QT>(aligned);
+  }
   if (nj <= 32) return gl_form<D, 4, 1, 2, 2, 2, 128, PT, QT>(aligned);
-  return gl_form<D, GL_BIG, PT, QT>(aligned);
+  if constexpr (!PT && !WIDE) {
+    if (nj >= 256 && rows / 256 * ((nj + 255) / 256) >= 512) return gl_form<D, 2, 4, 8, 4, 2, 128, PT, QT>(aligned);
+    return gl_form<D, 2, 2, 4, 4, 2, 128, PT, QT>(aligned);
+  }
+  return gl_form<D, 2, 2, 4, 4, 3, 64, PT, QT>(aligned);
 }
-template <bool PT, bool QT> static GlForm gl_pick_dtype(int dtype, int nj, bool aligned) {
-  return dtype == DGCNN_F32 ? gl_pick<DgF32, PT, QT>(nj, aligned) : dtype == DGCNN_BF16 ? gl_pick<DgBF16, PT, QT>(nj, aligned) : gl_pick<DgF16, PT, QT>(nj, aligned);
+template <bool PT, bool QT> static GlForm gl_pick_dtype(int dtype, int64_t rows, int E, int nj, bool aligned) {
+  return dtype == DGCNN_F32 ? gl_pick<DgF32, PT, QT>(rows, E, nj, aligned) : dtype == DGCNN_BF16 ? gl_pick<DgBF16, PT, QT>(rows, E, nj, aligned) : gl_pick<DgF16, PT, QT>(rows, E, nj, aligned);
 }
 static int gl_launch(const GlForm& f, int64_t blocks, const DgGl& a, hipStream_t s) {
   if (blocks <= 0) return DGCNN_OK;
@@ -525,7 +553,7 @@ static int gl_check(const dgcnn_grouped_linear_args* p) {
 
 extern "C" int64_t dgcnn_grouped_linear_workspace_bytes(int64_t rows, int in_features, int out_features, int groups, int dtype) {
   if (rows < 0 || in_features < 1 || out_features < 1 || groups < 0 || !dg_dtype_ok(dtype)) return DGCNN_EINVAL;
-  const GlForm f = gl_pick_dtype<true, true>(dtype, in_features, true);
+  const GlForm f = gl_pick_dtype<true, true>(dtype, rows, groups, in_features, true);
   const int64_t tiles = (int64_t)dg_cdiv(out_features, f.bi) * dg_cdiv(in_features, f.bj);
   const int shift = gl_slice(rows, groups, tiles);
   if (!shift) return 256;
@@ -544,9 +572,9 @@ extern "C" int dgcnn_grouped_linear_fwd(const dgcnn_grouped_linear_args* p, void
   a.p = p->x; a.q = p->weight; a.bias = p->bias; a.c = y; a.ptr = p->ptr; a.M = p->rows;
   a.ldp = p->ldx; a.ldq = p->in_features; a.ldc = p->out_features; a.qstride = (int64_t)p->in_features * p->out_features;
   a.ni = -1; a.nj = p->out_features; a.nr = p->in_features; a.E = p->groups;
-  const bool aligned = !((reinterpret_cast<uintptr_t>(p->x) | reinterpret_cast<uintptr_t>(p->weight) | reinterpret_cast<uintptr_t>(y)) & 15) &&
+  const bool aligned = !((reinterpret_cast<uintptr_t>(p->x) | reinterpret_cast<uintptr_t>(p->weight) | reinterpret_cast<uintptr_t>(p->bias) | reinterpret_cast<uintptr_t>(y)) & 15) &&
                        p->in_features % ce == 0 && p->ldx % ce == 0 && p->out_features % ce == 0;
-  const GlForm f = gl_pick_dtype<false, false>(p->dtype, a.nj, aligned);
+  const GlForm f = gl_pick_dtype<false, false>(p->dtype, p->rows, p->groups, a.nj, aligned);
   a.tj = dg_cdiv(a.nj, f.bj);
   return gl_launch(f, dg_align((p->rows / f.bi + p->groups + 2) * a.tj, 8), a, (hipStream_t)stream);
 }
@@ -565,7 +593,7 @@ extern "C" int dgcnn_grouped_linear_bwd(const dgcnn_grouped_linear_args* p, cons
     a.ldp = p->out_features; a.ldq = p->in_features; a.ldc = p->in_features; a.qstride = (int64_t)p->in_features * p->out_features;
     a.ni = -1; a.nj = p->in_features; a.nr = p->out_features; a.E = p->groups;
     const bool aligned = wide && !((reinterpret_cast<uintptr_t>(dy) | reinterpret_cast<uintptr_t>(p->weight) | reinterpret_cast<uintptr_t>(dx)) & 15);
-    const GlForm f = gl_pick_dtype<false, true>(p->dtype, a.nj, aligned);
+    const GlForm f = gl_pick_dtype<false, true>(p->dtype, p->rows, p->groups, a.nj, aligned);
     a.tj = dg_cdiv(a.nj, f.bj);
     const int r2 = gl_launch(f, dg_align((p->rows / f.bi + p->groups + 2) * a.tj, 8), a, (hipStream_t)stream);
     if (r2 != DGCNN_OK) return r2;
@@ -576,7 +604,7 @@ extern "C" int dgcnn_grouped_linear_bwd(const dgcnn_grouped_linear_args* p, cons
     a.ldp = p->out_features; a.ldq = p->ldx; a.ldc = p->in_features;
     a.ni = p->out_features; a.nj = p->in_features; a.nr = -1; a.E = p->groups;
     const bool aligned = wide && p->ldx % ce == 0 && !((reinterpret_cast<uintptr_t>(dy) | reinterpret_cast<uintptr_t>(p->x) | reinterpret_cast<uintptr_t>(dweight)) & 15);
-    const GlForm f = gl_pick_dtype<true, true>(p->dtype, a.nj, aligned);
+    const GlForm f = gl_pick_dtype<true, true>(p->dtype, p->rows, p->groups, a.nj, aligned);
     a.ti = dg_cdiv(a.ni, f.bi); a.tj = dg_cdiv(a.nj, f.bj);
     const int64_t tiles = (int64_t)a.ti * a.tj;
     a.shift = gl_slice(p->rows, p->groups, tiles);
@@ -584,7 +612,7 @@ extern "C" int dgcnn_grouped_linear_bwd(const dgcnn_grouped_linear_args* p, cons
     a.part = static_cast<float*>(ws);
     if (a.split && p->groups > 65535) return DGCNN_EUNSUPPORTED;
     a.slots = a.split ? (p->rows >> a.shift) + p->groups : 0;
-    const int r2 = gl_launch(f, (a.split ? a.slots : p->groups) * tiles, a, (hipStream_t)stream);
+    const int r2 = gl_launch(f, dg_align(a.split ? a.slots : p->groups, 8) * tiles, a, (hipStream_t)stream);
     if (r2 != DGCNN_OK) return r2;
     if (a.split) {
       const int64_t bx = (gl_each(a) / 4 + 255) / 256;
