@@ -495,9 +495,6 @@ k_gl_join(const DgGl a) {
   }
 }
 
-#ifndef GL_FEW
-#define GL_FEW 16
-#endif
 // ---- host ------------------------------------------------------------------------------------------------------------------------
 typedef void (*gl_kernel)(const DgGl);
 struct GlForm { gl_kernel k; int bi, bj, threads, lds; };
@@ -508,11 +505,19 @@ template <class D, int WI, int WJ, int FI, int FJ, int ST, int ROWB, bool PT, bo
   f.lds = ST * (f.bi + f.bj) * ROWB;
   return f;
 }
-// A tile for the shape (rows: of the whole call; nj: columns of C)
+// The tile for a shape (rows: of the whole call; nj: columns of C).  Measured, us, forward unless said:
+//   16 x 32, six stages: few rows, where the weights are the work and every workgroup has to stream its own share.  bf16, 8 groups, 1024 -> 1024: 48 rows 6.9 (128 x
+//     128: 12.9), 256 rows 8.4 (13.1), 512 rows 10.0 (13.3), 1024 rows 18.6 (14.5): up to 1024 tiles.  4096 -> 4096, 256 rows, 2048 tiles: 78 (60).  fp32, whose larger
+//     tiles multiply rows that are not there: 1024 rows 41 (78), 2048 rows 77 (79), 4096 -> 4096 256 rows 203 (295): up to 2048 tiles.
+//   128 x 32: narrow results.
+//   256 x 256, one workgroup a CU: 131072 rows 512 -> 512 bf16 116 (130), 1024 -> 512 178 (208), 8192 rows 4096 -> 4096 240 (294); but 16384 rows 4096 -> 512, 128 tiles
+//     of it, 108 (70): from two tiles a CU on.
+//   128 x 128 otherwise; 64 bytes of r in three stages (three workgroups a CU) for fp32 (97 -> 128 forward 63, 128 bytes in two stages 77) and dW (131, 138), 128 bytes in
+//     two for the others (16384 rows 4096 -> 512: 70, 87).
 template <class D, bool PT, bool QT> static GlForm gl_pick(int64_t rows, int E, int nj, bool aligned) {
   constexpr bool WIDE = sizeof(typename D::S) == 4;
   if constexpr (!PT) {
-    if (rows <= GL_FEW * (int64_t)E) return gl_form<D, 1, 2, 1, 1, 6, 128, PT, QT>(aligned);
+    if (rows <= 16 * (int64_t)E || (rows + 15) / 16 * ((nj + 31) / 32) <= (WIDE ? 2048 : 1024)) return gl_form<D, 1, 2, 1, 1, 6, 128, PT, QT>(aligned);
   }
   if (nj <= 32) return gl_form<D, 4, 1, 2, 2, 2, 128, PT, QT>(aligned);
   if constexpr (!PT && !WIDE) {

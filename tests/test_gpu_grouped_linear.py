@@ -117,6 +117,31 @@ def test_large(dtype, rows, groups, k, n):
 
 @gpu
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("k,n", [(40, 1024), (1024, 40), (33, 1030)])
+def test_many_rows_and_wide_results(dtype, k, n):
+    """enough tiles for the largest form, forward (wide out) and backward (wide in), with groups that end inside tiles and rows of none"""
+    if not torch.cuda.is_available():
+        pytest.skip("too large for the emulation")
+    ptr = torch.tensor([100, 9000, 9000, 9001, 31777, 33000])
+    x, w, b, dy = inputs(33300, 5, k, n, dtype)
+    check(x, w, b, ptr, dy)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("k,n", [(64, 96), (50, 33)])
+def test_between_few_rows_and_many(dtype, k, n):
+    """rows enough for the 128-row tiles at a width that keeps the emulation quick"""
+    ptr = torch.tensor([0, 700, 703, 2900])
+    if dtype == torch.float32:
+        n += 200
+    x, w, b, dy = inputs(2900 if torch.cuda.is_available() else 1500, 3, k, n, dtype)
+    ptr = ptr.clamp_max(x.shape[0])
+    check(x, w, b, ptr, dy)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_views_and_alignment(dtype):
     """rows with a stride, a start in the middle of a vector, a transposed x, an int32 ptr, an expanded dy, no bias"""
     x, w, b, dy = inputs(70, 3, 16, 24, dtype)
