@@ -372,7 +372,13 @@ class AdamW(Optimizer):
     def load_state_dict(self, state_dict) -> None:
         """As ``Optimizer.load_state_dict``, but every tensor of the state keeps its own type (torch's casts them to the parameter's, which codes, scales
         and the float32 moments of 16-bit parameters do not survive)."""
+        for g in state_dict["param_groups"]:
+            if g.get("amsgrad") or g.get("maximize"):
+                raise ValueError("dgcnn_amd.optim.AdamW has no amsgrad or maximize variant: this state is another optimizer's")
         super().load_state_dict(state_dict)
+        for g in self.param_groups:              # (torch's groups hold no state_bits, master_weights, seed)
+            for k, v in self.defaults.items():
+                g.setdefault(k, v)
         saved = list(chain.from_iterable(g["params"] for g in state_dict["param_groups"]))
         mine = list(chain.from_iterable(g["params"] for g in self.param_groups))
         for k, p in zip(saved, mine):

@@ -266,7 +266,8 @@ def test_state_of_torchs_adamw_loads():
         p.grad = g
         a.step()
     q.data.copy_(p.data)
-    b.load_state_dict({"state": a.state_dict()["state"], "param_groups": b.state_dict()["param_groups"]})
+    b.load_state_dict(a.state_dict())
+    assert b.param_groups[0]["state_bits"] == 32 and b.param_groups[0]["lr"] == 1e-2
     for o, x in ((a, p), (b, q)):
         x.grad = g
         o.step()
@@ -403,6 +404,13 @@ def test_constructor_refusals():
     for kw in (dict(amsgrad=True), dict(state_bits=16), dict(lr=-1.0), dict(betas=(0.9, 1.0)), dict(eps=-1e-8), dict(weight_decay=-0.1), dict(lr=torch.tensor(1e-3))):
         with pytest.raises(ValueError):
             optim.AdamW(p, **kw)
+
+
+def test_states_of_other_variants_are_refused():
+    p = [torch.nn.Parameter(torch.zeros(3))]
+    for kw in (dict(amsgrad=True), dict(maximize=True)):
+        with pytest.raises(ValueError):
+            optim.AdamW(p).load_state_dict(torch.optim.AdamW(p, **kw).state_dict())
 
 
 def test_c_entry_refuses_bad_arguments():
