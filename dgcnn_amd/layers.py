@@ -91,7 +91,7 @@ def graph_ptr(data) -> torch.Tensor:
 def _grouped_args(x, weight, bias, ptr):
     rows, fin = x.shape
     groups, fout = weight.shape[:2]
-    return _lib.GroupedLinearArgs(rows, max(x.stride(0), fin), fin, fout, groups, _DTYPES[x.dtype], x.data_ptr(), weight.data_ptr(),
+    return _lib.GroupedLinearArgs(rows, x.stride(0) if rows > 1 else fin, fin, fout, groups, _DTYPES[x.dtype], x.data_ptr(), weight.data_ptr(),
                                   None if bias is None else bias.data_ptr(), ptr.data_ptr())
 
 
@@ -147,7 +147,7 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, ptr: torch.Tensor, bia
     ptr = _check_ptr(ptr, x)
     if ptr.numel() != weight.shape[0] + 1:
         _no(f"ptr must be [{weight.shape[0] + 1}] for {weight.shape[0]} groups, got [{ptr.numel()}]")
-    if x.stride(1) != 1 or (x.shape[0] > 1 and x.stride(0) < x.shape[1]):      # (rows may be strided; anything else is copied)
+    if x.stride(1) != 1 or (x.shape[0] > 1 and not x.shape[1] <= x.stride(0) <= 1 << 21):      # (rows may be strided; anything else is copied)
         x = x.contiguous()
     weight = weight.contiguous()
     bias = None if bias is None else bias.contiguous()
@@ -176,6 +176,12 @@ class GroupedLinear(nn.Module):
 
 
 # ---- group norm ----------------------------------------------------------------------------------------------------------------------
+def _norm_args(head, x, weight, bias, ptr, stats):
+    at = stats.data_ptr()
+    return _lib.GroupNormArgs(*head, x.data_ptr(), None if weight is None else weight.data_ptr(), None if bias is None else bias.data_ptr(),
+                              None if ptr is None else ptr.data_ptr(), at, at + 2 * stats.numel())
+
+
 def _norm_forward(x, weight, bias, ptr, groups, eps, act):
     C = x.shape[-1]
     segments = x.shape[0] if ptr is None else ptr.numel() - 1
@@ -185,35 +191,32 @@ def _norm_forward(x, weight, bias, ptr, groups, eps, act):
     y = torch.empty_like(x) if segments else torch.zeros_like(x)
     stats = torch.empty(2, segments, groups, dtype=torch.float32, device=x.device)
     ws = torch.empty(_bytes("dgcnn_group_norm_workspace_bytes", rows, C, groups, segments, ptr is None, dtype, 0), dtype=torch.uint8, device=x.device)
-    at = stats.data_ptr()
-    args = (rows, C, groups, segments, dtype, 0 if some is None else _DTYPES[some.dtype], act, eps, 0, x.data_ptr(),
-            None if weight is None else weight.data_ptr(), None if bias is None else bias.data_ptr(), None if ptr is None else ptr.data_ptr(),
-            at, at + 4 * segments * groups)
-    _launch(_lib.lib().dgcnn_group_norm_fwd, "dgcnn_group_norm_fwd", x.device, ctypes.byref(_lib.GroupNormArgs(*args)), y.data_ptr(), ws.data_ptr())
-    return y, stats, args
+    head = (rows, C, groups, segments, dtype, 0 if some is None else _DTYPES[some.dtype], act, eps, 0)
+    _launch(_lib.lib().dgcnn_group_norm_fwd, "dgcnn_group_norm_fwd", x.device, ctypes.byref(_norm_args(head, x, weight, bias, ptr, stats)), y.data_ptr(),
+            ws.data_ptr())
+    return y, stats, head
 
 
 class _GroupNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, ptr, groups, eps, act):
-        y, stats, ctx.args = _norm_forward(x, weight, bias, ptr, groups, eps, act)
-        ctx.save_for_backward(x, weight, bias, ptr, stats)      # (args hold the addresses of these)
+        y, stats, ctx.head = _norm_forward(x, weight, bias, ptr, groups, eps, act)
+        ctx.save_for_backward(x, weight, bias, ptr, stats)
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
         x, weight, bias, ptr, stats = ctx.saved_tensors
-        args = ctx.args
-        rows, C, groups, segments, dtype = args[:5]
+        rows, C, groups, segments, dtype = ctx.head[:5]
         if not dy.is_contiguous():
             dy = dy.contiguous()
         dx = torch.empty_like(x) if segments else torch.zeros_like(x)
         dw = torch.empty_like(weight) if ctx.needs_input_grad[1] else None
         db = torch.empty_like(bias) if ctx.needs_input_grad[2] else None
         ws = torch.empty(_bytes("dgcnn_group_norm_workspace_bytes", rows, C, groups, segments, ptr is None, dtype, 1), dtype=torch.uint8, device=x.device)
-        _launch(_lib.lib().dgcnn_group_norm_bwd, "dgcnn_group_norm_bwd", x.device, ctypes.byref(_lib.GroupNormArgs(*args)), dy.data_ptr(), dx.data_ptr(),
-                None if dw is None else dw.data_ptr(), None if db is None else db.data_ptr(), ws.data_ptr())
+        _launch(_lib.lib().dgcnn_group_norm_bwd, "dgcnn_group_norm_bwd", x.device, ctypes.byref(_norm_args(ctx.head, x, weight, bias, ptr, stats)),
+                dy.data_ptr(), dx.data_ptr(), None if dw is None else dw.data_ptr(), None if db is None else db.data_ptr(), ws.data_ptr())
         return dx, dw, db, None, None, None, None
 
 

@@ -291,6 +291,36 @@ def test_forward_and_backward_in_a_graph_with_other_groups_at_each_replay(dtype)
 
 
 @gpu
+def test_the_largest_form_in_a_graph():
+    """128 KB of LDS, which is asked for at the call, also where the call is captured"""
+    if not torch.cuda.is_available():
+        pytest.skip("graphs need the GPU")
+    x, w, b, _ = (t.cuda() for t in inputs(33000, 2, 64, 1024, torch.bfloat16))
+    ptr = torch.tensor([0, 20000, 33000], device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = layers.grouped_linear(x, w, ptr, b)
+    for p in ([0, 20000, 33000], [0, 1, 32999], [300, 300, 33000]):
+        ptr.copy_(torch.tensor(p))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, layers.grouped_linear(x, w, ptr, b)), p
+
+
+@gpu
+def test_rows_of_unusual_strides():
+    """one row with any stride, rows too far apart for 32-bit offsets, expanded rows: as if contiguous"""
+    x, w, b, _ = (t.to("cuda") for t in inputs(3, 1, 16, 8, torch.float32))
+    ptr = torch.tensor([0, 3]).to("cuda")
+    far = torch.zeros(2, 1 << 22).to("cuda")
+    far[:, :16] = x[:2]
+    want = layers.grouped_linear(x, w, ptr, b)
+    assert torch.equal(layers.grouped_linear(far[:, :16], w, ptr.clamp_max(2), b), want[:2])
+    assert torch.equal(layers.grouped_linear(far[:1, :16], w, ptr.clamp_max(1), b), want[:1])
+    assert torch.equal(layers.grouped_linear(x[:1].expand(3, 16), w, ptr, b), want[:1].expand(3, 8))
+
+
+@gpu
 def test_refusals_on_device_tensors():
     x, w, b, _ = (t.to("cuda") for t in inputs(10, 2, 6, 4, torch.float32))
     ptr = torch.tensor([0, 4, 10]).to("cuda")

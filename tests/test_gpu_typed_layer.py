@@ -134,3 +134,25 @@ def test_example_in_bf16_runs_and_has_gradients():
     start = [p.detach().clone() for p in m.parameters()]
     o.step()
     assert any(not torch.equal(a, p.detach()) for a, p in zip(start, m.parameters()))
+
+
+@gpu
+@pytest.mark.parametrize("op", ["norm", "linear"])
+def test_backward_reads_what_saved_tensor_hooks_return(op):
+    """saved tensors may be moved between the passes (offloaded and brought back): the backward takes them where they are then"""
+    g = torch.Generator().manual_seed(2)
+    ptr = torch.tensor([0, 4, 4, 9]).to("cuda")
+    x0 = torch.randn(9, 8, generator=g)
+    w0 = torch.randn(8, generator=g) if op == "norm" else torch.randn(3, 5, 8, generator=g)
+    dy = torch.randn(9, 8 if op == "norm" else 5, generator=g).to("cuda")
+    got = []
+    for moved in (False, True):
+        x, w = (t.clone().to("cuda").requires_grad_(True) for t in (x0, w0))
+        with torch.autograd.graph.saved_tensors_hooks((lambda t: t.detach().clone()) if moved else (lambda t: t), lambda t: t):
+            y = layers.group_norm(x, 2, w, ptr=ptr, act="silu") if op == "norm" else layers.grouped_linear(x, w, ptr)
+        if moved:
+            x.data.zero_()
+            w.data.zero_()
+        got.append(torch.autograd.grad(y, (x, w), dy))
+    for a, b in zip(*got):
+        assert torch.equal(a, b) and bool(a.abs().max() > 0)
