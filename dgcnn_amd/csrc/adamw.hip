@@ -59,6 +59,7 @@ static __host__ __device__ inline DgAdamwScalars aw_scalars(double lr, double b1
 
 // the step counter lives on the device (captured training steps): count, and leave this step's factors for the launches behind
 __global__ void k_adamw_tick(int64_t* step, const float* lr_dev, double lr, double b1, double b2, double eps, double wd, DgAdamwScalars* out) {
+  if (threadIdx.x) return;      // (one wave, one lane of it)
   const int64_t t = *step + 1;
   *step = t;
   *out = aw_scalars(lr_dev ? (double)*lr_dev : lr, b1, b2, eps, wd, t);
@@ -257,7 +258,7 @@ extern "C" int dgcnn_adamw_step(const dgcnn_adamw_args* a, dgcnn_stream_t stream
   DgAdamwScalars sc = {};
   DgAdamwScalars* const dev = a->step_dev ? reinterpret_cast<DgAdamwScalars*>(a->scalars_dev) : nullptr;
   if (dev) {
-    hipLaunchKernelGGL(k_adamw_tick, dim3(1), dim3(1), 0, st, a->step_dev, a->lr_dev, a->lr, a->beta1, a->beta2, a->eps, a->weight_decay, dev);
+    hipLaunchKernelGGL(k_adamw_tick, dim3(1), dim3(64), 0, st, a->step_dev, a->lr_dev, a->lr, a->beta1, a->beta2, a->eps, a->weight_decay, dev);
     DG_CHECK_LAUNCH();
   } else {
     sc = aw_scalars(a->lr, a->beta1, a->beta2, a->eps, a->weight_decay, a->step);

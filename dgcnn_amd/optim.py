@@ -332,7 +332,8 @@ class AdamW(Optimizer):
     the bytes; the state then holds ``exp_avg``, ``exp_avg_sq`` (codes of the mean and of the root of the mean square) and their ``_scale`` tensors.
     ``master_weights``: bfloat16 / float16 parameters get a float32 copy (``master`` in the state) that carries the updates too small for their type.
     ``capturable``: the step counter lives on the device and ``step()`` may be captured into a graph; ``lr`` may then be a float32 device tensor of one
-    element.  A parameter without a gradient is left alone; ``seed`` picks the random rounding of 8-bit moments."""
+    element; parameters that were captured together share their counter, so eager steps beside the graph have to be for all of them.  A parameter without
+    a gradient is left alone; ``seed`` picks the random rounding of 8-bit moments."""
 
     def __init__(self, params, lr: Union[float, torch.Tensor] = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2, amsgrad: bool = False, *,
                  state_bits: int = 32, master_weights: bool = False, capturable: bool = False, seed: int = 0):
@@ -365,6 +366,7 @@ class AdamW(Optimizer):
             st["master"] = p.detach().to(torch.float32, copy=True)
         t = st["step"]
         if group["capturable"] != isinstance(t, torch.Tensor) or (group["capturable"] and (t.dtype != torch.int64 or t.device != p.device)):
+            _refuse(_capturing(), "run a step() after loading a state and before capturing one: its counters are not on the device yet")
             n = int(t)              # (a state of another kind was loaded: torch's counters are float32 tensors)
             st["step"] = fresh.setdefault((p.device, n), torch.full((1,), n, dtype=torch.int64, device=p.device)) if group["capturable"] else n
         return st
@@ -384,6 +386,10 @@ class AdamW(Optimizer):
         for k, p in zip(saved, mine):
             for name, v in state_dict["state"].get(k, {}).items():
                 if isinstance(v, torch.Tensor):
+                    if name != "step" and v.shape == p.shape and not v.is_contiguous() == p.is_contiguous():
+                        if v.dtype.itemsize == 1:
+                            raise ValueError("the 8-bit state of a parameter of another memory layout: its blocks are other elements")
+                        v = torch.empty_like(p, dtype=v.dtype).copy_(v)
                     # (counters come back as host numbers: step() makes one device counter for all equal ones)
                     self.state[p][name] = int(v) if name == "step" else v.detach().to(p.device, copy=True)
 
@@ -404,8 +410,21 @@ class AdamW(Optimizer):
                     g = torch.empty_like(p, dtype=g.dtype).copy_(g)
                 st = self._state_of(p, group, fresh)
                 t = st["step"]
-                calls.setdefault((p.device, p.dtype, g.dtype, "master" in st, t.data_ptr() if group["capturable"] else t), []).append((p, g, st))
+                calls.setdefault((p.device, p.dtype, g.dtype, "master" in st, t.data_ptr() if group["capturable"] else t, "exp_avg_scale" in st),
+                                 []).append((p, g, st))
             if group["capturable"]:
+                idle = {}                         # parameters that sit this step out keep their count
+                for p in group["params"]:
+                    t = self.state[p].get("step") if p.grad is None and p in self.state else None
+                    if isinstance(t, torch.Tensor):
+                        idle.setdefault(t.data_ptr(), []).append(self.state[p])
+                for items in calls.values():
+                    t = items[0][2]["step"]
+                    if t.data_ptr() in idle:
+                        _refuse(_capturing(), "run a step() with gradients for the same parameters before capturing one")
+                        t = t.clone()
+                        for st in idle.pop(items[0][2]["step"].data_ptr()):
+                            st["step"] = t
                 counted = set()
                 for items in calls.values():      # a call counts its counter up: no two calls may share one
                     t = items[0][2]["step"]

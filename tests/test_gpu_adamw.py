@@ -406,6 +406,44 @@ def test_constructor_refusals():
             optim.AdamW(p, **kw)
 
 
+@gpu
+@pytest.mark.parametrize("capturable", [False, True])
+def test_parameters_without_gradients_keep_their_count(capturable):
+    """b has a gradient in two steps of three: its bias corrections are those of its own second step"""
+    init = [torch.linspace(-1, 1, 300), torch.linspace(1, 2, 70)]
+    ours = [torch.nn.Parameter(t.clone().to("cuda")) for t in init]
+    plain = [torch.nn.Parameter(t.double()) for t in init]
+    a, b = optim.AdamW(ours, lr=1e-2, capturable=capturable), torch.optim.AdamW(plain, lr=1e-2)
+    for k in range(3):
+        for i, (p, q) in enumerate(zip(ours, plain)):
+            g = None if (i, k) == (1, 1) else torch.randn(p.shape, generator=torch.Generator().manual_seed(10 * k + i))
+            p.grad, q.grad = (None, None) if g is None else (g.to("cuda"), g.double())
+        a.step(); b.step()
+    assert [int(a.state[p]["step"]) for p in ours] == [3, 2]
+    for p, q in zip(ours, plain):      # three steps of a few roundings of values up to 2, and of updates up to 1e-2 a step
+        assert (p.detach().cpu().double() - q.detach()).abs().max() <= 3 * 4 * 2.0 * 2 ** -24
+
+
+@gpu
+def test_states_load_into_parameters_of_another_layout():
+    x = torch.randn(4, 3, 5, 5, generator=torch.Generator().manual_seed(3))
+    p, q = (torch.nn.Parameter(x.clone().to("cuda").contiguous(memory_format=f)) for f in (torch.contiguous_format, torch.channels_last))
+    a, b = optim.AdamW([p]), optim.AdamW([q])
+    for _ in range(2):
+        p.grad = torch.ones_like(p) * x.to("cuda")
+        a.step()
+    q.data.copy_(p.data)
+    b.load_state_dict(a.state_dict())
+    for o, t in ((a, p), (b, q)):
+        t.grad = torch.empty_like(t).copy_(x)
+        o.step()
+    assert torch.equal(p, q) and torch.equal(a.state[p]["exp_avg"], b.state[q]["exp_avg"])
+    small = optim.AdamW([p], state_bits=8)
+    small.step()
+    with pytest.raises(ValueError):
+        optim.AdamW([q], state_bits=8).load_state_dict(small.state_dict())
+
+
 def test_states_of_other_variants_are_refused():
     p = [torch.nn.Parameter(torch.zeros(3))]
     for kw in (dict(amsgrad=True), dict(maximize=True)):
