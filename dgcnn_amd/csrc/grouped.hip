@@ -531,7 +531,7 @@ template <bool PT, bool QT> static GlForm gl_pick_dtype(int dtype, int64_t rows,
 }
 static int gl_launch(const GlForm& f, int64_t blocks, const DgGl& a, hipStream_t s) {
   if (blocks <= 0) return DGCNN_OK;
-  if (blocks > 0x7fffffff) return DGCNN_EUNSUPPORTED;
+  if (blocks > 0xffffffffll / f.threads) return DGCNN_EUNSUPPORTED;      // (a grid holds fewer than 2^32 threads)
   if (f.lds > 64 * 1024 && hipFuncSetAttribute(reinterpret_cast<const void*>(f.k), hipFuncAttributeMaxDynamicSharedMemorySize, f.lds) != hipSuccess) return DGCNN_ELAUNCH;
   hipLaunchKernelGGL(f.k, dim3((unsigned)blocks), dim3(f.threads), f.lds, s, a);
   DG_CHECK_LAUNCH();

@@ -24,6 +24,7 @@
 // (w, b, the sums of dw and db) spills
 static constexpr int gn_most(int vec) { return vec >= 4 ? 512 : 1024; }
 #define GN_WROWS 2048        // workgroups of a role that keep dw / db sums (rows of partial sums)
+#define GN_MOST (1 << 17)    // workgroups of a role in the forward pass: a grid holds fewer than 2^32 threads
 #define GN_MAX_D 2048        // channels of a group
 
 struct DgGn {
@@ -673,7 +674,7 @@ static void gn_grid(DgGn* a, int es, bool bwd) {
   // for each sum out of the caches.
   a->L = a->N * a->C * es <= 512 * 1024 && (a->ptr ? a->N : a->per) > a->R ? a->N : a->R;
   const bool one_long = (a->ptr ? a->N : a->per) > a->L;      // can any segment be longer?
-  a->nseg = one_long && !a->ptr ? 0 : bwd && a->B > GN_WROWS ? GN_WROWS : a->B;      // (dense samples: all or none)
+  a->nseg = one_long && !a->ptr ? 0 : a->B > (bwd ? GN_WROWS : GN_MOST) ? (bwd ? GN_WROWS : GN_MOST) : a->B;      // (dense samples: all or none)
   a->nchunk = one_long ? (int)((a->N + a->R - 1) / a->R) : 0;
   const int most = bwd ? 1024 : 2048;      // (backward: a row of partial sums each)
   a->cgrid = a->nchunk < most ? a->nchunk : most;
@@ -683,6 +684,10 @@ static bool gn_shape(DgGn* a, int64_t rows, int C, int groups, int segments) {
   a->N = rows; a->B = segments; a->C = C; a->G = groups; a->D = C / groups;
   return true;
 }
+// counts of 32 bits: chunks hold at least 2^10 of 2^40 elements, the join takes 16 threads a (segment, group)
+static bool gn_fits(const DgGn& a) {
+  return a.N <= ((int64_t)1 << 40) / a.C && a.C <= 1 << 24 && (int64_t)a.B * a.G <= 1 << 27;
+}
 static int64_t gn_part_bytes(const DgGn& a) { return a.nchunk ? dg_align(((int64_t)a.nchunk + a.B) * a.G * 2 * 4, 256) : 0; }
 static int64_t gn_ac_bytes(const DgGn& a) { return a.nchunk ? dg_align((int64_t)a.B * a.G * 2 * 4, 256) : 0; }
 
@@ -691,7 +696,7 @@ extern "C" int64_t dgcnn_group_norm_workspace_bytes(int64_t rows, int C, int gro
   DgGn a = {};
   if (!gn_shape(&a, rows, C, groups, segments) || !dg_dtype_ok(dtype)) return DGCNN_EINVAL;
   if (segments == 0 || rows == 0) return 256;
-  if (rows > ((int64_t)1 << 40) / C) return DGCNN_EUNSUPPORTED;
+  if (!gn_fits(a)) return DGCNN_EUNSUPPORTED;
   static const int64_t dummy[2] = {0, 0};
   int64_t most = 256;
   for (int cap = 8; cap >= 1; cap >>= 1) {
@@ -744,7 +749,7 @@ static int gn_check(const dgcnn_group_norm_args* p, DgGn* a) {
   if (p->rows > 0 && p->segments > 0 && (!p->x || !p->mean || !p->rstd)) return DGCNN_EINVAL;
   if (!p->ptr && p->segments > 0 && p->rows % p->segments) return DGCNN_EINVAL;
   if (!p->ptr && p->segments == 0 && p->rows > 0) return DGCNN_EINVAL;
-  if (p->rows > ((int64_t)1 << 40) / p->channels) return DGCNN_EUNSUPPORTED;
+  if (!gn_fits(*a)) return DGCNN_EUNSUPPORTED;
   a->x = p->x; a->w = p->weight; a->b = p->bias; a->ptr = p->ptr; a->mean = p->mean; a->rstd = p->rstd;
   a->per = !p->ptr && p->segments ? p->rows / p->segments : 0;
   a->wdt = p->weight_dtype; a->act = p->act; a->eps = p->eps;
@@ -762,6 +767,7 @@ extern "C" int dgcnn_group_norm_fwd(const dgcnn_group_norm_args* p, void* y, voi
   const int cap = gn_vec_cap(reinterpret_cast<uintptr_t>(p->x) | reinterpret_cast<uintptr_t>(y), a.C, dg_dtype_size(p->dtype));
   if (!gn_plan(&a, p->dtype, cap, false, &vec, &threads, &tiles)) return DGCNN_EUNSUPPORTED;
   gn_grid(&a, dg_dtype_size(p->dtype), false);
+  if ((int64_t)a.nchunk * threads >> 32) return DGCNN_EUNSUPPORTED;
   a.part = static_cast<float*>(ws);
   hipLaunchKernelGGL(gn_pick_dtype(p->dtype, vec, a.L > a.R ? GN_FWD_STREAM : GN_FWD), dim3(a.nseg + a.cgrid, tiles), dim3(threads), 0, (hipStream_t)stream, a);
   DG_CHECK_LAUNCH();
@@ -793,6 +799,7 @@ extern "C" int dgcnn_group_norm_bwd(const dgcnn_group_norm_args* p, const void* 
   const int cap = gn_vec_cap(reinterpret_cast<uintptr_t>(p->x) | reinterpret_cast<uintptr_t>(dy) | reinterpret_cast<uintptr_t>(dx), a.C, dg_dtype_size(p->dtype));
   if (!gn_plan(&a, p->dtype, cap, true, &vec, &threads, &tiles)) return DGCNN_EUNSUPPORTED;
   gn_grid(&a, dg_dtype_size(p->dtype), true);
+  if ((int64_t)a.nchunk * threads >> 32) return DGCNN_EUNSUPPORTED;
   a.part = static_cast<float*>(ws);
   char* const after = static_cast<char*>(ws) + gn_part_bytes(a);
   a.ac = reinterpret_cast<float*>(after);

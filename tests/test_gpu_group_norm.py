@@ -325,6 +325,23 @@ def test_forward_and_backward_in_a_graph():
 
 
 @gpu
+def test_more_segments_than_workgroups():
+    if not torch.cuda.is_available():
+        pytest.skip("2^17 workgroups take the emulation minutes")
+    n = (1 << 17) + 77
+    x = torch.randn(n, 2, 4, generator=torch.Generator().manual_seed(5)).cuda()
+    y = layers.group_norm(x, 2, act="tanh")
+    ptr = torch.arange(0, 2 * n + 1, 2, device="cuda")
+    assert torch.equal(y.view(-1, 4), layers.group_norm(x.view(-1, 4), 2, ptr=ptr, act="tanh"))
+    d = x.double().view(n, 2, 2, 2)      # [sample, row, group, channel]
+    want = torch.tanh((d - d.mean((1, 3), keepdim=True)) / (d.var((1, 3), correction=0, keepdim=True) + 1e-5).sqrt()).view(n, 2, 4)
+    # (|h| <= sqrt(3) for four values; a difference of two values near each other and its root: 16 roundings of the largest value, over a deviation of at
+    # least sqrt(eps))
+    bound = 16 * 2.0 ** -24 * (1 + d.abs().amax((1, 3), keepdim=True) / (d.var((1, 3), correction=0, keepdim=True) + 1e-5).sqrt())
+    assert bool(((y.double() - want).view(n, 2, 2, 2).abs() <= bound).all())
+
+
+@gpu
 def test_refusals_on_device_tensors():
     x, w, b, _ = (t.to("cuda") for t in inputs(10, 12, torch.float32))
     ptr = torch.tensor([0, 4, 10]).to("cuda")
@@ -377,3 +394,15 @@ def test_c_entries_refuse_bad_arguments():
     ask = L.dgcnn_group_norm_workspace_bytes
     assert ask(100, 8, 2, 3, 0, 0, 1) > 0 and ask(0, 8, 2, 0, 1, 0, 0) > 0
     assert ask(-1, 8, 2, 3, 0, 0, 1) == -1 and ask(4, 8, 3, 3, 0, 0, 1) == -1 and ask(4, 8, 2, 2, 0, 7, 1) == -1
+
+
+def test_counts_beyond_the_grids_are_refused():
+    import ctypes
+    L = _lib.lib()
+    buf = (ctypes.c_float * 64)()
+    at = ctypes.addressof(buf)
+    for kw in (dict(channels=1 << 25, groups=1 << 25), dict(segments=1 << 28, rows=1 << 28)):
+        a = _lib.GroupNormArgs(**{**dict(rows=4, channels=8, groups=2, segments=2, eps=1e-5, x=at, mean=at, rstd=at), **kw})
+        assert L.dgcnn_group_norm_fwd(ctypes.byref(a), at, at, None) == -3
+        assert L.dgcnn_group_norm_bwd(ctypes.byref(a), at, at, None, None, at, None) == -3
+        assert L.dgcnn_group_norm_workspace_bytes(a.rows, a.channels, a.groups, a.segments, 1, 0, 0) == -3
