@@ -12,7 +12,7 @@
 //   * a longer segment is the business of the chunks it spans: each leaves its partial (mean, M2) per group -- slot = chunk + segment, unique
 //     because (chunk, segment) pairs form a staircase -- and a second launch combines the partials of the segment (a few KB, from L2) and
 //     reads its chunk once more (from the last-level cache when the tensor fits it).
-// Lengths are known on the device alone, so both run in ONE launch (workgroups 0..segments-1 and the chunks behind them), and the second launch
+// Lengths are known on the device alone, so both run in ONE launch (the workgroups of whole segments and, behind them, those of the chunks), and the second launch
 // is left out when the host knows that no segment can be longer than L (few rows, or equal lengths).  Nothing is summed by atomics: every
 // sum has one order.
 // A thread keeps one column (VEC channels of one group) and every RY-th row; sums over a group go through one LDS slot a thread.
@@ -23,8 +23,7 @@
 // ... and at most, which is also how many vectors a group may be wide: 1024 threads leave 128 registers each, which wide vectors' arithmetic
 // (w, b, the sums of dw and db) spills
 static constexpr int gn_most(int vec) { return vec >= 4 ? 512 : 1024; }
-#define GN_WROWS 2048        // workgroups of a role that keep dw / db sums (rows of partial sums)
-#define GN_MOST (1 << 17)    // workgroups of a role in the forward pass: a grid holds fewer than 2^32 threads
+#define GN_CUS 256           // compute units
 #define GN_MAX_D 2048        // channels of a group
 
 struct DgGn {
@@ -375,9 +374,13 @@ k_gn_fwd(const DgGn a) {
 }
 
 // ---- long segments: the partials of a segment's chunks, then its rows once more -----------------------------------------------------
-// 16 lanes a (segment, group).  Forward: mean = sum n_i mean_i / n, M2 = sum M2_i + n_i (mean_i - mean)^2 -> mean, rstd.  Backward: the two means -> ac.
-template <bool BWD> __device__ __forceinline__ void gn_join(const DgGn& a, int64_t item) {
-  const int l = threadIdx.x & 15, s = (int)(item / a.G), g = (int)(item % a.G);
+// 64 lanes a (segment, group) where there are at most 4096 of them, else 16 (backward, with the sum of dw and db: 512 of 256 partials 5.2 us, with 16 lanes
+// 9.9; 16384, most of them of none, 7.9 and 6.3).  Forward: mean = sum n_i mean_i / n, M2 = sum M2_i + n_i (mean_i - mean)^2 -> mean, rstd.  Backward: the two means -> ac.
+__host__ __device__ inline int gn_join_lanes(const DgGn& a) { return (int64_t)a.B * a.G <= 4096 ? 64 : 16; }
+template <bool BWD> __device__ __forceinline__ void gn_join(const DgGn& a, int64_t thread) {
+  const int lanes = gn_join_lanes(a), l = (int)thread & (lanes - 1);
+  const int64_t item = thread / lanes;
+  const int s = (int)(item / a.G), g = (int)(item % a.G);
   int64_t lo = 0, hi = 0;
   if (s < a.B) {
     if (a.ptr) { lo = min(max(a.ptr[s], (int64_t)0), a.N); hi = min(max(a.ptr[s + 1], lo), a.N); }
@@ -390,8 +393,8 @@ template <bool BWD> __device__ __forceinline__ void gn_join(const DgGn& a, int64
   float u = 0.f, v = 0.f;
   if (BWD) {
 #pragma unroll 4
-    for (int i = l; i < n; i += 16) { u += p[(int64_t)i * a.G * 2]; v += p[(int64_t)i * a.G * 2 + 1]; }
-    u = gn_lanes(u, 16); v = gn_lanes(v, 16);
+    for (int i = l; i < n; i += lanes) { u += p[(int64_t)i * a.G * 2]; v += p[(int64_t)i * a.G * 2 + 1]; }
+    u = gn_lanes(u, lanes); v = gn_lanes(v, lanes);
     if (on && l == 0) {
       a.ac[((int64_t)s * a.G + g) * 2] = u / (rows * (float)a.D);
       a.ac[((int64_t)s * a.G + g) * 2 + 1] = v / (rows * (float)a.D);
@@ -399,22 +402,22 @@ template <bool BWD> __device__ __forceinline__ void gn_join(const DgGn& a, int64
     return;
   }
 #pragma unroll 4
-  for (int i = l; i < n; i += 16)
+  for (int i = l; i < n; i += lanes)
     u += p[(int64_t)i * a.G * 2] * (float)(min((int64_t)(k0 + i + 1) * a.R, hi) - max((int64_t)(k0 + i) * a.R, lo));
-  u = gn_lanes(u, 16);
+  u = gn_lanes(u, lanes);
   const float m = u / rows;
 #pragma unroll 4
-  for (int i = l; i < n; i += 16) {
+  for (int i = l; i < n; i += lanes) {
     const float d = p[(int64_t)i * a.G * 2] - m;
     v += p[(int64_t)i * a.G * 2 + 1] + (float)(min((int64_t)(k0 + i + 1) * a.R, hi) - max((int64_t)(k0 + i) * a.R, lo)) * (float)a.D * d * d;
   }
-  v = gn_lanes(v, 16);
+  v = gn_lanes(v, lanes);
   if (on && l == 0) {
     a.mean[(int64_t)s * a.G + g] = m;
     a.rstd[(int64_t)s * a.G + g] = 1.f / sqrtf(v / rows / (float)a.D + a.eps);
   }
 }
-__global__ void __launch_bounds__(256) k_gn_join(const DgGn a) { gn_join<false>(a, (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4)); }
+__global__ void __launch_bounds__(256) k_gn_join(const DgGn a) { gn_join<false>(a, (int64_t)blockIdx.x * 256 + threadIdx.x); }
 
 // rows [at0, at1) of long segment s; ROWS(at, left) for each R of them
 template <class F> __device__ __forceinline__ void gn_long_rows(const DgGn& a, int k, F rows) {
@@ -617,14 +620,14 @@ __global__ void __launch_bounds__(1024)
 k_gn_wsum(const DgGn a, int rows, int wblocks, void* dw, void* db, int dt) {
   __shared__ float red[128][9];
   if ((int)blockIdx.x >= wblocks) {
-    gn_join<true>(a, (int64_t)(blockIdx.x - wblocks) * 64 + (threadIdx.x >> 4));
+    gn_join<true>(a, (int64_t)(blockIdx.x - wblocks) * 1024 + threadIdx.x);
     return;
   }
   const int c = threadIdx.x & 7, col = blockIdx.x * 8 + c, lane = threadIdx.x >> 3;
   float s = 0.f;
   if (col < 2 * a.C) {
     const float* const p = a.wpart + col;
-#pragma unroll 8
+#pragma unroll 16
     for (int r = lane; r < rows; r += 128) s += p[(int64_t)r * 2 * a.C];
   }
   red[lane][c] = s;
@@ -674,17 +677,20 @@ static void gn_grid(DgGn* a, int es, bool bwd) {
   // for each sum out of the caches.
   a->L = a->N * a->C * es <= 512 * 1024 && (a->ptr ? a->N : a->per) > a->R ? a->N : a->R;
   const bool one_long = (a->ptr ? a->N : a->per) > a->L;      // can any segment be longer?
-  a->nseg = one_long && !a->ptr ? 0 : a->B > (bwd ? GN_WROWS : GN_MOST) ? (bwd ? GN_WROWS : GN_MOST) : a->B;      // (dense samples: all or none)
+  // Workgroups of a role: three of 256 threads fit a compute unit backward (141 registers), four forward.  Up to four each, one item a workgroup; beyond
+  // that as many as fit at once, each with a contiguous share or every cgrid-th chunk.  2048 graphs of 128 bf16 channels: backward 41 us with 768, 45 with 1024,
+  // 49 with 2048 (and the sum of their partial rows 6, 7, 9); forward 25.6 with 1024, 27.9 with 2048; 16 x 4096 rows of 512: backward 35, 42 with 1024, forward 16.4, 18.7.
+  const int all = GN_CUS * 4, most = GN_CUS * (bwd ? 3 : 4);
+  a->nseg = one_long && !a->ptr ? 0 : a->B <= all ? a->B : most;      // (dense samples: all or none)
   a->nchunk = one_long ? (int)((a->N + a->R - 1) / a->R) : 0;
-  const int most = bwd ? 1024 : 2048;      // (backward: a row of partial sums each)
-  a->cgrid = a->nchunk < most ? a->nchunk : most;
+  a->cgrid = a->nchunk <= all ? a->nchunk : most;
 }
 static bool gn_shape(DgGn* a, int64_t rows, int C, int groups, int segments) {
   if (rows < 0 || C < 1 || groups < 1 || C % groups || segments < 0) return false;
   a->N = rows; a->B = segments; a->C = C; a->G = groups; a->D = C / groups;
   return true;
 }
-// counts of 32 bits: chunks hold at least 2^10 of 2^40 elements, the join takes 16 threads a (segment, group)
+// counts of 32 bits: chunks hold at least 2^10 of 2^40 elements, the joins take 16 threads a (segment, group)
 static bool gn_fits(const DgGn& a) {
   return a.N <= ((int64_t)1 << 40) / a.C && a.C <= 1 << 24 && (int64_t)a.B * a.G <= 1 << 27;
 }
@@ -772,7 +778,7 @@ extern "C" int dgcnn_group_norm_fwd(const dgcnn_group_norm_args* p, void* y, voi
   hipLaunchKernelGGL(gn_pick_dtype(p->dtype, vec, a.L > a.R ? GN_FWD_STREAM : GN_FWD), dim3(a.nseg + a.cgrid, tiles), dim3(threads), 0, (hipStream_t)stream, a);
   DG_CHECK_LAUNCH();
   if (a.cgrid) {
-    hipLaunchKernelGGL(k_gn_join, dim3((unsigned)(((int64_t)a.B * a.G + 15) / 16)), dim3(256), 0, (hipStream_t)stream, a);
+    hipLaunchKernelGGL(k_gn_join, dim3((unsigned)(((int64_t)a.B * a.G * gn_join_lanes(a) + 255) / 256)), dim3(256), 0, (hipStream_t)stream, a);
     DG_CHECK_LAUNCH();
     hipLaunchKernelGGL(gn_pick_dtype(p->dtype, vec, GN_FWD_LONG), dim3(a.nchunk, tiles), dim3(threads), 0, (hipStream_t)stream, a);
     DG_CHECK_LAUNCH();
@@ -807,7 +813,7 @@ extern "C" int dgcnn_group_norm_bwd(const dgcnn_group_norm_args* p, const void* 
   hipLaunchKernelGGL(gn_pick_dtype(p->dtype, vec, a.L > a.R ? GN_BWD_STREAM : GN_BWD), dim3(a.nseg + a.cgrid, tiles), dim3(threads), 0, (hipStream_t)stream, a);
   DG_CHECK_LAUNCH();
   const int wblocks = a.wpart ? dg_cdiv(2 * a.C, 8) : 0;
-  const int64_t jblocks = a.cgrid ? ((int64_t)a.B * a.G + 63) / 64 : 0;
+  const int64_t jblocks = a.cgrid ? ((int64_t)a.B * a.G * gn_join_lanes(a) + 1023) / 1024 : 0;
   if (wblocks + jblocks) {
     hipLaunchKernelGGL(k_gn_wsum, dim3((unsigned)(wblocks + jblocks)), dim3(1024), 0, (hipStream_t)stream, a, a.nseg + a.cgrid, wblocks, dweight, dbias, p->weight_dtype);
     DG_CHECK_LAUNCH();

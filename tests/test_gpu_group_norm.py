@@ -325,9 +325,23 @@ def test_forward_and_backward_in_a_graph():
 
 
 @gpu
+@pytest.mark.parametrize("long_rows", [0, 5000, 300000])
+def test_workgroups_that_walk_several_segments_and_chunks(long_rows):
+    """1100 graphs are more than the workgroups of a role, and so are the chunks of a long one among them"""
+    if long_rows > 5000 and not torch.cuda.is_available():
+        pytest.skip("too long for the emulation")
+    g = torch.Generator().manual_seed(11)
+    lens = torch.randint(0, 4, (1100,), generator=g)
+    if long_rows:
+        lens[700] = long_rows
+    ptr = torch.cat([torch.zeros(1, dtype=torch.int64), lens.cumsum(0)])
+    check(*inputs(int(ptr[-1]) + 2, 32, torch.float32, seed=4), ptr, 4, "silu")
+
+
+@gpu
 def test_more_segments_than_workgroups():
     if not torch.cuda.is_available():
-        pytest.skip("2^17 workgroups take the emulation minutes")
+        pytest.skip("2^17 segments take the emulation minutes")
     n = (1 << 17) + 77
     x = torch.randn(n, 2, 4, generator=torch.Generator().manual_seed(5)).cuda()
     y = layers.group_norm(x, 2, act="tanh")
