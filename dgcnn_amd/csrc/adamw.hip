@@ -88,7 +88,7 @@ __device__ __forceinline__ uint32_t aw_encode(float t, uint32_t noise16) {
   code = a < 512.f ? code : 127u;                                     // (NaN)
   return code | ((__float_as_uint(t) >> 24) & 0x80u);
 }
-__device__ __forceinline__ uint32_t aw_hash(uint32_t h) {             // the 32-bit finalizer of MurmurHash3 (Appleby, public domain)
+__device__ __forceinline__ uint32_t aw_hash(uint32_t h) {             // a bijective 32-bit mixer of xor-shifts and odd multipliers (constants in the public domain)
   h = (h ^ (h >> 16)) * 0x85EBCA6Bu;
   h = (h ^ (h >> 13)) * 0xC2B2AE35u;
   return h ^ (h >> 16);
