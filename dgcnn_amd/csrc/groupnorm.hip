@@ -17,6 +17,10 @@
 // sum has one order.
 // A thread keeps one column (VEC channels of one group) and every RY-th row; sums over a group go through one LDS slot a thread.
 // Statistics, partials and dw / db sums are fp32; y and dx are rounded once.
+// Measured (MI355X; a 1 GiB copy reaches 5.2 TB/s): 16 maps of 64 x 64 x 512 bf16, 32 groups, silu, 67 MB a tensor: forward 16 us (reads x, 4.2 TB/s) + 4.5 (join) + 25
+// (reads x, writes y, 5.4 TB/s), backward 35 (3.8 TB/s) + 5 + 37 (5.4 TB/s).  2048 graphs of 74 rows on average, 128 bf16 channels, 8 groups, silu, 39 MB a tensor:
+// forward 26 + 5 + 11, backward 41 + 6.5 + 22: short segments leave a workgroup's loads and its sums one after the other, three or four workgroups a
+// compute unit hide part of it.  3725 rows of 32 fp32 channels, 50 graphs: 8.5 us, one launch.
 #include "dg_half.h"
 
 #define GN_T 256             // threads of a workgroup, at least
