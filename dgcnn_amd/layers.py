@@ -176,6 +176,12 @@ class GroupedLinear(nn.Module):
 
 
 # ---- group norm ----------------------------------------------------------------------------------------------------------------------
+def _wide(t, channels: int):
+    """contiguous, and aligned where a group's channels only fit a workgroup as vectors"""
+    t = t.contiguous()
+    return t.clone() if channels > 1024 and t.data_ptr() & 15 else t
+
+
 def _norm_args(head, x, weight, bias, ptr, stats):
     at = stats.data_ptr()
     return _lib.GroupNormArgs(*head, x.data_ptr(), None if weight is None else weight.data_ptr(), None if bias is None else bias.data_ptr(),
@@ -209,8 +215,7 @@ class _GroupNorm(torch.autograd.Function):
     def backward(ctx, dy):
         x, weight, bias, ptr, stats = ctx.saved_tensors
         rows, C, groups, segments, dtype = ctx.head[:5]
-        if not dy.is_contiguous():
-            dy = dy.contiguous()
+        dy = _wide(dy, C // groups)
         dx = torch.empty_like(x) if segments else torch.zeros_like(x)
         dw = torch.empty_like(weight) if ctx.needs_input_grad[1] else None
         db = torch.empty_like(bias) if ctx.needs_input_grad[2] else None
@@ -227,7 +232,7 @@ def group_norm(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tensor] 
 
     ``ptr`` None: ``x`` is ``[B, ..., C]`` and a sample is everything behind the first dimension.  Otherwise ``x`` is ``[N, C]`` and sample ``s`` is rows
     ``ptr[s] .. ptr[s + 1] - 1`` (ascending, on the device; never read by the host); samples may be empty, rows outside every sample give 0 and
-    get gradient 0.  ``act``: "none", "relu", "silu", "gelu" (with erf) or "tanh".  ``weight`` and ``bias`` may be of another type than ``x``;
+    get gradient 0.  A group has at most 1024 channels (2048 if even).  ``act``: "none", "relu", "silu", "gelu" (with erf) or "tanh".  ``weight`` and ``bias`` may be of another type than ``x``;
     ``y`` is of ``x``'s.  Differentiable once in ``x``, ``weight`` and ``bias``."""
     if act not in ACTS:
         _no(f"act must be one of {sorted(ACTS)}, got {act!r}")
@@ -254,7 +259,7 @@ def group_norm(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tensor] 
         if x.dim() != 2:
             _no(f"with ptr, x must be [N, C], got {tuple(x.shape)}")
         ptr = _check_ptr(ptr, x)
-    x = x.contiguous()
+    x = _wide(x, C // num_groups)
     weight, bias = (None if t is None else t.contiguous() for t in (weight, bias))
     if not _wants_grad(x, weight, bias):
         return _norm_forward(x, weight, bias, ptr, num_groups, eps, ACTS[act])[0]

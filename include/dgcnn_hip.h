@@ -395,7 +395,7 @@ int dgcnn_grouped_linear_bwd(const dgcnn_grouped_linear_args* args, const void* 
  * outside [0, rows], gives unspecified values, never an access outside the tensors.)  segments 0: y and dx are not written.
  * weight, bias [channels] of weight_dtype, each may be NULL (1 and 0).  mean, rstd [segments, groups] fp32: written by _fwd, read by _bwd.
  * x, y, dy, dx are of dtype; dweight and dbias (each may be NULL) of weight_dtype.  Channels of a group: at most 1024 in
- * any case, 2048 if even (tensors 8-byte aligned), else DGCNN_EUNSUPPORTED.
+ * any case, 2048 if even (tensors 8-byte aligned), else DGCNN_EUNSUPPORTED; as beyond 2^40 elements, 2^24 channels or 2^27 (segment, group) pairs.
  * ws: dgcnn_group_norm_workspace_bytes(rows, channels, groups, segments, ptr == NULL, dtype, backward) bytes. */
 #define DGCNN_ACT_NONE 0
 #define DGCNN_ACT_RELU 1

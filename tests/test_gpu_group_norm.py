@@ -339,6 +339,25 @@ def test_workgroups_that_walk_several_segments_and_chunks(long_rows):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_the_widest_groups_at_odd_addresses(dtype):
+    """2048 channels fit a workgroup as vectors only: tensors that are not aligned for them are copied"""
+    x, w, b, dy = inputs(5, 2048, dtype, seed=6)
+    ptr = torch.tensor([0, 2, 5])
+
+    def odd(t):
+        v = torch.empty(t.numel() + 1, dtype=t.dtype, device="cuda" if torch.cuda.is_available() else "cpu")[1:].view(t.shape)
+        return v.copy_(t)
+
+    X, W, B = odd(x).requires_grad_(True), w.to("cuda").requires_grad_(True), b.to("cuda").requires_grad_(True)
+    y = layers.group_norm(X, 1, W, B, ptr=ptr.to("cuda"), act="silu")
+    got = (y, *torch.autograd.grad(y, (X, W, B), odd(dy)))
+    for p, q in zip(got, run(x, w, b, dy, ptr, 1, "silu")):
+        assert torch.equal(p, q)
+    check(x, w, b, dy, ptr, 1, "silu")
+
+
+@gpu
 def test_more_segments_than_workgroups():
     if not torch.cuda.is_available():
         pytest.skip("2^17 segments take the emulation minutes")
