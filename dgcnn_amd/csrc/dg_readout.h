@@ -45,9 +45,7 @@ __device__ __forceinline__ void dg_select_topk(const float* __restrict__ x4, int
     // (this thread's first key is requested BEFORE the barrier, unconditionally on a clamped node: behind it the load was a round
     //  trip of its own in front of the LDS store)
     const float k0 = x4[n0 + max(min(tid, n - 1), 0)];
-#ifndef RD_TOPK_NO_ENTRY_BARRIER      // (measurement: callers that placed a full barrier right in front of this function do not need it)
     dg_lds_barrier();
-#endif
     SK_MARK(1);
     if (tid < npad) keys[tid] = tid < n ? dg_pack_key(k0, tid) : ~0ull;
     for (int t = tid + T; t < npad; t += T) keys[t] = t < n ? dg_pack_key(x4[n0 + t], t) : ~0ull;

@@ -964,9 +964,7 @@ ch_chain_body(int N, int B, int F, const int* __restrict__ sched, const int* __r
     // One tile per wave (!TWO): conv4 reads nothing the next staging writes -- its bitmap words are in registers (`wreg`, read
     // behind the staging barrier, and every wave has passed three more barriers since), h4p / dv alternate with `par`, the image H
     // was last read in conv3's product in front of the barrier at CH_T(8), the tables are constant -> no barrier needed.
-#ifndef CH_NO_LOOP_END_BARRIER      // (the unsafe form exists only to show that the race-delay test catches its absence: profiles/r06_race_test.txt)
     if (LOOP && TWO) dg_lds_barrier();
-#endif
     n0 = n0N; n = nN; par ^= 1;
   }
 #ifdef CH_TIMING
@@ -2087,9 +2085,7 @@ k_chain_bwd_a(int N, int B, const int* __restrict__ sched, const int* __restrict
         }
       }
     }
-#ifndef CH_NO_LOOP_END_BARRIER
     if (LOOP) dg_lds_barrier();      // (conv3's product reads `bl` word by word and the loop top re-stages `bl`: see ch_chain_body's loop end; k_chain_bwd_b has the same barrier)
-#endif
     n0 = n0N; n = nN; par ^= 1;
   }
   // ---- this workgroup's partial rows: the waves' accumulators combined in a fixed order ---------------------------------------

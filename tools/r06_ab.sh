@@ -1,6 +1,6 @@
 #!/bin/bash
 # A/B of the step-kernel candidates (docs/rounds/r06.md): parity tests, quick bench line and phase table per variant library
-# usage (GPU box): bash tools/r06_ab.sh wpre1 noeb ...      (variants built by tools/build_variant.sh; `default` is always run first)
+# usage (GPU box): bash tools/r06_ab.sh wpre1 ...      (variants built by tools/build_variant.sh; `default` is always run first)
 exec < /dev/null
 R=${GRAFT_REPO_ROOT:-/root/repo}; cd $R; O=gpurun_out; mkdir -p $O
 Q="--min-seconds 1 --no-cpu-baseline --no-pmc --large-batch 0 --no-dropin --steps 400 --warmup 40"
