@@ -7,8 +7,8 @@
 //
 // Bound: HBM (forward x in, y out; backward x and dy in, dx out).  The tensor is cut into CHUNKS of R rows, R such that a workgroup holds a
 // chunk in registers (NV vectors a thread), and every row is read once into registers, whatever the segments' lengths:
-//   * a segment of at most R rows belongs to one workgroup: read once, statistics over the registers (mean first, then the squares
-//     of the differences: no cancellation), written once (a form of the kernel for small tensors streams any length: L, not R, is where a segment counts as long);
+//   * a segment of at most R rows belongs to one workgroup: read once, statistics over the registers, written once (a form of the kernel for
+//     small tensors streams any length: L, not R, is where a segment counts as long);
 //   * a longer segment is the business of the chunks it spans: each leaves its partial (mean, M2) per group -- slot = chunk + segment, unique
 //     because (chunk, segment) pairs form a staircase -- and a second launch combines the partials of the segment (a few KB, from L2) and
 //     reads its chunk once more (from the last-level cache when the tensor fits it).
@@ -17,6 +17,11 @@
 // sum has one order.
 // A thread keeps one column (VEC channels of one group) and every RY-th row; sums over a group go through one LDS slot a thread.
 // Statistics, partials and dw / db sums are fp32; y and dx are rounded once.
+// Mean and M2 = sum (x - mean)^2 take two sums: m = sum x / n, off by up to K 2^-24 mean|x| after K rounded additions in a row; then, over t = x - m (exact
+// where x is near m), S1 = sum t and S2 = sum t^2:  mean = m + S1 / n,  M2 = S2 - S1^2 / n.  What m was off by is in S1, so the mean is left with its
+// own rounding: a constant segment's mean is the constant, and small noise on a large offset keeps its variance.  K stays below 200
+// forward, 280 backward: a thread sums its 64 (backward 8 a channel) elements of a piece, then the pieces' sums, LDS adds up to 32 and 6 more.  Most pieces: 512 KB of
+// 129 16-bit channels, one a thread, 127 of 16 rows forward and 254 of 8 backward.
 // Measured (MI355X; a 1 GiB copy reaches 5.2 TB/s): 16 maps of 64 x 64 x 512 bf16, 32 groups, silu, 67 MB a tensor: forward 16 us (reads x, 4.2 TB/s) + 4.5 (join) + 25
 // (reads x, writes y, 5.4 TB/s), backward 35 (3.8 TB/s) + 5 + 37 (5.4 TB/s).  2048 graphs of 74 rows on average, 128 bf16 channels, 8 groups, silu, 39 MB a tensor:
 // forward 26 + 5 + 11, backward 41 + 6.5 + 22: short segments leave a workgroup's loads and its sums one after the other, three or four workgroups a
@@ -228,7 +233,8 @@ template <class F> __device__ __forceinline__ void gn_pieces(const DgGn& a, int6
   for (int64_t at = lo; at < hi; at += a.R) f(at, (int)min(hi - at, (int64_t)a.R));
 }
 
-// x - mu is kept apart from the scale: a constant segment gives exactly b, and a large mean cancels before anything is rounded.  rw = rstd * w.
+// x - mu is kept apart from the scale: a constant segment, whose mean is the constant, gives exactly b, and a large mean cancels before anything is
+// rounded.  rw = rstd * w.
 template <class D, int VEC> __device__ __forceinline__ DgRaw<D, VEC> gn_apply(const DgGn& a, const DgRaw<D, VEC>& v, float mu, const float* rw, const float* b) {
   float z[VEC];
   DgRaw<D, VEC> o;
@@ -303,7 +309,7 @@ k_gn_fwd(const DgGn a) {
   })) {
     const int left = (int)min(it.hi - it.lo, (int64_t)a.R);
     const float n = (float)(it.hi - it.lo) * (float)a.D;
-    float sum = 0.f, sq = 0.f;
+    float sum = 0.f, t1 = 0.f, t2 = 0.f;
     if constexpr (!STREAM) {
       gn_load<D, VEC, NV>(a, me, x, it.lo, left, v);
 #pragma unroll
@@ -314,45 +320,56 @@ k_gn_fwd(const DgGn a) {
       gn_pieces(a, it.lo, it.hi, [&](int64_t at, int left) {
         DgRaw<D, VEC> u[NV];
         gn_load<D, VEC, NV>(a, me, x, at, left, u);
+        float s = 0.f;
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) sum += u[i].get(e);
+          for (int e = 0; e < VEC; ++e) s += u[i].get(e);
+        sum += s;
       });
     }
     gn_sum<false>(a, L, me, gn, sum, 0.f);
     if constexpr (!STREAM) dg_hide<D, VEC, NV>(v);
-    const float mu = me.on ? L.stat[0][me.g] / n : 0.f;      // (divided: a constant segment's mean is the constant, its squares' sum 0)
+    float mu = me.on ? L.stat[0][me.g] / n : 0.f;
     if constexpr (!STREAM) {
 #pragma unroll
       for (int i = 0; i < NV; ++i)
         if (me.r < left - i * a.RY) {
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) { const float d = v[i].get(e) - mu; sq += d * d; }
+          for (int e = 0; e < VEC; ++e) { const float t = v[i].get(e) - mu; t1 += t; t2 += t * t; }
         }
     } else {
       gn_pieces(a, it.lo, it.hi, [&](int64_t at, int left) {
         DgRaw<D, VEC> u[NV];
         gn_load<D, VEC, NV>(a, me, x, at, left, u);
+        float s1 = 0.f, s2 = 0.f;
 #pragma unroll
         for (int i = 0; i < NV; ++i)
           if (me.r < left - i * a.RY) {
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) { const float d = u[i].get(e) - mu; sq += d * d; }
+            for (int e = 0; e < VEC; ++e) { const float t = u[i].get(e) - mu; s1 += t; s2 += t * t; }
           }
+        t1 += s1; t2 += s2;
       });
     }
-    gn_sum<false>(a, L, me, gn, sq, 0.f);
+    gn_sum<true>(a, L, me, gn, t1, t2);
+    float m2 = 0.f;
+    if (me.on) {
+      const float off = L.stat[0][me.g] / n;
+      mu += off;
+      m2 = L.stat[1][me.g] - L.stat[0][me.g] * off;
+      m2 = m2 < 0.f ? 0.f : m2;      // (rounding, where all of S2 was m's error; NaN stays)
+    }
     if constexpr (!STREAM) dg_hide<D, VEC, NV>(v);
     const bool first = me.r == 0 && me.c == me.g * a.DV;      // one thread of each group
     if (it.slot >= 0) {
       if (first) {
         float* const p = a.part + ((int64_t)it.slot * a.G + g0 + me.g) * 2;
-        p[0] = mu; p[1] = L.stat[0][me.g];
+        p[0] = mu; p[1] = m2;
       }
       continue;
     }
-    const float rs = me.on ? 1.f / sqrtf(L.stat[0][me.g] / n + a.eps) : 0.f;
+    const float rs = me.on ? 1.f / sqrtf(m2 / n + a.eps) : 0.f;
     if (first) { a.mean[(int64_t)it.s * a.G + g0 + me.g] = mu; a.rstd[(int64_t)it.s * a.G + g0 + me.g] = rs; }
     float rw[VEC];
 #pragma unroll
@@ -379,7 +396,8 @@ k_gn_fwd(const DgGn a) {
 
 // ---- long segments: the partials of a segment's chunks, then its rows once more -----------------------------------------------------
 // 64 lanes a (segment, group) where there are at most 4096 of them, else 16 (backward, with the sum of dw and db: 512 of 256 partials 5.2 us, with 16 lanes
-// 9.9; 16384, most of them of none, 7.9 and 6.3).  Forward: mean = sum n_i mean_i / n, M2 = sum M2_i + n_i (mean_i - mean)^2 -> mean, rstd.  Backward: the two means -> ac.
+// 9.9; 16384, most of them of none, 7.9 and 6.3).  Forward: mean = mean_0 + sum n_i (mean_i - mean_0) / n (equal means stay what they are), M2 = sum M2_i +
+// n_i (mean_i - mean)^2 -> mean, rstd.  Backward: the two means -> ac.
 __host__ __device__ inline int gn_join_lanes(const DgGn& a) { return (int64_t)a.B * a.G <= 4096 ? 64 : 16; }
 template <bool BWD> __device__ __forceinline__ void gn_join(const DgGn& a, int64_t thread) {
   const int lanes = gn_join_lanes(a), l = (int)thread & (lanes - 1);
@@ -405,11 +423,12 @@ template <bool BWD> __device__ __forceinline__ void gn_join(const DgGn& a, int64
     }
     return;
   }
+  const float m0 = on ? p[0] : 0.f;
 #pragma unroll 4
   for (int i = l; i < n; i += lanes)
-    u += p[(int64_t)i * a.G * 2] * (float)(min((int64_t)(k0 + i + 1) * a.R, hi) - max((int64_t)(k0 + i) * a.R, lo));
+    u += (p[(int64_t)i * a.G * 2] - m0) * (float)(min((int64_t)(k0 + i + 1) * a.R, hi) - max((int64_t)(k0 + i) * a.R, lo));
   u = gn_lanes(u, lanes);
-  const float m = u / rows;
+  const float m = m0 + u / rows;
 #pragma unroll 4
   for (int i = l; i < n; i += lanes) {
     const float d = p[(int64_t)i * a.G * 2] - m;
@@ -539,14 +558,19 @@ k_gn_bwd(const DgGn a) {
         DgRaw<D, VEC> d[NV];
         gn_load<D, VEC, NV>(a, me, x, at, left, v);
         gn_load<D, VEC, NV>(a, me, dy, at, left, d);
+        float pq[VEC], pqt[VEC];      // (the piece's sums apart: fewer additions in a row)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) pq[e] = pqt[e] = 0.f;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
           if (me.r < left - i * a.RY) {
             gn_q<D, VEC>(a, v[i], d[i], mu, rw, b, q[i]);
-            gn_add<D, VEC>(v[i], mu, q[i], sq, sqt);
+            gn_add<D, VEC>(v[i], mu, q[i], pq, pqt);
           }
           GN_FENCE();
         }
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) { sq[e] += pq[e]; sqt[e] += pqt[e]; }
       });
     }
     float s1 = 0.f, s2 = 0.f;
