@@ -16,6 +16,7 @@ from typing import Optional
 
 import torch
 from torch import nn
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -74,6 +75,9 @@ def _check_ptr(ptr: torch.Tensor, x: torch.Tensor) -> torch.Tensor:
 
 
 def _wants_grad(*ts) -> bool:
+    """Whether autograd has to see the call.  For a forward-mode tangent, which no_grad does not switch off, it raises there: the functions have no rule for it."""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in ts):
+        return True
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
 
 
