@@ -293,8 +293,9 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
         _refuse(True, f"betas must lie in [0, 1) and eps must not be negative, got {betas}, {eps}")
 
     a = _lib.AdamwArgs()
-    keep = None
+    keep, counter = None, ()
     if isinstance(step, torch.Tensor):
+        counter = (step,)
         _refuse(step.dtype != torch.int64 or step.numel() != 1 or step.device != dev, f"step must be an int or an int64 tensor of one element on {dev}")
         keep = torch.empty(16, dtype=torch.float32, device=dev)
         a.step_dev, a.scalars_dev = step.data_ptr(), keep.data_ptr()
@@ -323,6 +324,8 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
     with contextlib.nullcontext() if dev.index is None or dev.index == torch.cuda.current_device() else torch.cuda.device(dev):
         rc = _lib.lib().dgcnn_adamw_step(ctypes.byref(a), torch._C._cuda_getCurrentRawStream(dev.index))
     _lib.check(rc, "dgcnn_adamw_step")
+    # (the library writes through addresses: what a graph saved of these has to count as changed)
+    torch.autograd.graph.increment_version(chain(params, exp_avgs, exp_avg_sqs, masters or (), exp_avg_scales or (), exp_avg_sq_scales or (), counter))
 
 
 class AdamW(Optimizer):
