@@ -230,22 +230,34 @@ _numel, _is_contiguous, _get_device, _data_ptr = (getattr(torch.Tensor, k) for k
 _get_dtype = operator.attrgetter("dtype")
 
 
+def _layout(t):
+    """how a tensor's elements lie in memory: sizes and strides of the dimensions that have more than one"""
+    return [(n, s) for n, s in zip(t.shape, t.stride()) if n != 1]
+
+
+def _dense(t) -> bool:
+    """every place from the first element to the last one holds exactly one, in whatever order"""
+    if t.is_contiguous():
+        return True
+    want = 1
+    for n, s in sorted(_layout(t), key=operator.itemgetter(1)):
+        if s != want:
+            return False
+        want *= n
+    return True
+
+
 def _check_list(name, ts, params, numels, device, dtypes) -> torch.dtype:
     """Every tensor of one of `dtypes`, as large and laid out as its parameter (or, for scales, `numels` contiguous elements); the type."""
     # (a few C loops over the whole list; the tensors are looked at one by one only to say which it is)
     kinds = set(map(_get_dtype, ts))
     if len(ts) == len(numels) and len(kinds) == 1 and kinds <= dtypes and set(map(_get_device, ts)) == device and list(map(_numel, ts)) == numels and \
             (all(map(_is_contiguous, ts)) and (params is None or all(map(_is_contiguous, params)))
-             or params is not None and all(t.stride() == p.stride() for t, p in zip(ts, params))):
+             or params is not None and all(_layout(t) == _layout(p) for t, p in zip(ts, params))):
         return kinds.pop()
     raise _lib.DgcnnError(f"{name} must be {len(numels)} tensors of one type ({', '.join(sorted(map(str, dtypes)))}) on one device, "
                           + (f"contiguous with one element for each {STATE_BLOCK} of the parameter" if params is None else "with their parameters' sizes and strides")
                           + f"; got {len(ts)}: " + ", ".join(f"{t.dtype} {tuple(t.shape)} {t.stride()} on {t.device}" for t in list(ts)[:4]))
-
-
-def _dense(p) -> bool:
-    return p.is_contiguous() or (p.dim() == 4 and p.is_contiguous(memory_format=torch.channels_last)) or \
-        (p.dim() == 5 and p.is_contiguous(memory_format=torch.channels_last_3d))
 
 
 def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], exp_avgs: Sequence[torch.Tensor], exp_avg_sqs: Sequence[torch.Tensor], *,
@@ -256,7 +268,8 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
 
         m = b1 m + (1 - b1) g      v = b2 v + (1 - b2) g^2      p = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
 
-    ``params`` are of one type (float32, bfloat16, float16), dense, and no two of them share memory; ``grads`` of the same type, or float32.
+    ``params`` are of one type (float32, bfloat16, float16), dense (contiguous in some order of their dimensions, which the other lists follow), and no two of
+    them share memory; ``grads`` of the same type, or float32.
     Moments are float32, or -- with both scale lists -- 8 bits: ``exp_avgs`` and ``exp_avg_sqs`` then are ``torch.float8_e4m3fn`` codes of ``m`` and of
     ``sqrt(v)``, each times one float32 scale for 256 consecutive elements (``[ceil(numel / 256)]``).  Codes are rounded stochastically by a hash of
     (``seed``, tensor, step, element), so that the means do not stall between two codes; equal arguments give equal bits.
@@ -273,7 +286,7 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
     numels, device = list(map(_numel, params)), {p0.get_device()}
     kind = _check_list("params", params, params, numels, device, _DTYPES.keys())
     if not all(map(_is_contiguous, params)) and not all(map(_dense, params)):
-        _refuse(True, "parameters must be dense tensors")
+        _refuse(True, "parameters must be dense tensors: contiguous in some order of their dimensions")
     bits = 32 if exp_avg_scales is None else 8
     if (exp_avg_scales is None) != (exp_avg_sq_scales is None):
         _refuse(True, "8-bit moments need both exp_avg_scales and exp_avg_sq_scales")
@@ -329,7 +342,7 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
 
 
 class AdamW(Optimizer):
-    """``torch.optim.AdamW`` (no amsgrad) over GPU parameters of any layout: one launch for each 48 tensors of a type.
+    """``torch.optim.AdamW`` (no amsgrad) over GPU parameters of any dense layout: one launch for each 48 tensors of a type.
 
     ``state_bits`` 32: float32 moments, ``state_dict()`` as torch's (and torch's loads).  8: moments as :func:`adamw_step` describes them, a quarter of
     the bytes; the state then holds ``exp_avg``, ``exp_avg_sq`` (codes of the mean and of the root of the mean square) and their ``_scale`` tensors.
@@ -389,7 +402,7 @@ class AdamW(Optimizer):
         for k, p in zip(saved, mine):
             for name, v in state_dict["state"].get(k, {}).items():
                 if isinstance(v, torch.Tensor):
-                    if name != "step" and v.shape == p.shape and not v.is_contiguous() == p.is_contiguous():
+                    if name != "step" and v.shape == p.shape and _layout(v) != _layout(p):
                         if v.dtype.itemsize == 1:
                             raise ValueError("the 8-bit state of a parameter of another memory layout: its blocks are other elements")
                         v = torch.empty_like(p, dtype=v.dtype).copy_(v)
@@ -409,7 +422,7 @@ class AdamW(Optimizer):
                 if g is None:
                     continue
                 _refuse(g.is_sparse, "dgcnn_amd.optim.AdamW takes dense gradients")
-                if g.stride() != p.stride() and _dense(p):
+                if g.stride() != p.stride() and _layout(g) != _layout(p) and _dense(p):
                     g = torch.empty_like(p, dtype=g.dtype).copy_(g)
                 st = self._state_of(p, group, fresh)
                 t = st["step"]
