@@ -14,7 +14,7 @@ from ctypes import c_char_p, c_double, c_float, c_int, c_int64, c_uint64, c_void
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("DGCNN_HIP_LIB") or os.path.join(_HERE, "libdgcnn_hip.so")   # env override: A/B experiments
 CSRC = os.path.join(_HERE, "csrc")
-ABI_VERSION = 21
+ABI_VERSION = 22
 FLAG_COALESCED_UNDIRECTED = 1
 FLAG_FORCE_FUSED = 2
 FLAG_FORCE_TILED = 4
@@ -74,7 +74,7 @@ class AdamwArgs(ctypes.Structure):
                 ("step", c_int64), ("step_dev", c_void_p), ("lr_dev", c_void_p), ("scalars_dev", c_void_p),
                 ("seed", c_uint64), ("first_index", c_int64),
                 ("param_dtype", ctypes.c_int32), ("grad_dtype", ctypes.c_int32), ("state_bits", ctypes.c_int32), ("count", ctypes.c_int32),
-                ("tensors", c_void_p)]
+                ("tensors", c_void_p), ("indices", c_void_p)]
 
 
 class GroupNormArgs(ctypes.Structure):

@@ -11,14 +11,15 @@
 // largest magnitude is code 448).  r instead of v: e4m3 spans a factor of 2^17 in r, 2^35 in v.  An element with v > 0 never gets code 0:
 // its next update would divide by eps alone.  Codes are rounded STOCHASTICALLY (up with the probability of the distance from the
 // lower neighbour): b2 = 0.999 changes r by at most 1/2000 of its value in a step while half a code step is 3..6 %, so rounding to nearest would
-// leave r where it is from its tenth step on, a factor of ~10 too small.  The random bits are a hash of (seed, tensor, step, element),
-// so a step is reproducible.  The update itself uses m and v before they are rounded.
+// leave r where it is from its tenth step on, a factor of ~10 too small.  The random bits are a hash of (seed, the tensor's index,
+// step, element), so a step is reproducible.  The update itself uses m and v before they are rounded.
 // NaN and infinities are coded as NaN and leave the block's scale to its finite elements.
 //
 // Measured (MI355X; a 1 GiB copy reaches 5.2 TB/s): 200 M fp32 elements in 40 tensors 1034 us, 5.4 TB/s; 24 M bf16 ones with fp32 copies and moments in 60 tensors (two
 // launches) 140 us, 4.8 TB/s; 200 M bf16 ones with 8-bit moments 490 us, 4.1 TB/s, held back by the arithmetic of decoding, scaling, hashing and encoding
 // two codes an element; 16 tensors of 52 K elements together 5.4 us, a launch's own time.
-// The operation sequence is fixed (no contraction): a step's result does not depend on alignment, on the list a tensor is in, or on the launch.
+// The operation sequence is fixed (no contraction): a step's result does not depend on alignment, on the list a tensor is in, or on the launch (with 8-bit
+// moments: as long as the tensor keeps its index).
 #include "dg_half.h"
 #include <math.h>
 
@@ -282,7 +283,7 @@ extern "C" int dgcnn_adamw_step(const dgcnn_adamw_args* a, dgcnn_stream_t stream
     const bool end = i == a->count;
     if (!end && a->tensors[i].numel > 0) {
       const dgcnn_adamw_tensor* t = &a->tensors[i];
-      uint64_t z = a->seed + 0x9E3779B97F4A7C15ull * (uint64_t)(a->first_index + i + 1);      // (splitmix64, as the dropout mask's)
+      uint64_t z = a->seed + 0x9E3779B97F4A7C15ull * ((uint64_t)(a->indices ? a->indices[i] : a->first_index + i) + 1);      // (splitmix64, as the dropout mask's)
       z = (z ^ (z >> 30)) * 0xBF58476D1CE4E5B9ull;
       z = (z ^ (z >> 27)) * 0x94D049BB133111EBull;
       tab.param[k] = t->param; tab.grad[k] = t->grad; tab.m[k] = t->exp_avg; tab.v[k] = t->exp_avg_sq;

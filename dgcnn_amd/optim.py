@@ -263,7 +263,8 @@ def _check_list(name, ts, params, numels, device, dtypes) -> torch.dtype:
 def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], exp_avgs: Sequence[torch.Tensor], exp_avg_sqs: Sequence[torch.Tensor], *,
                step: Union[int, torch.Tensor], lr: Union[float, torch.Tensor] = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2,
                masters: Optional[Sequence[torch.Tensor]] = None, exp_avg_scales: Optional[Sequence[torch.Tensor]] = None,
-               exp_avg_sq_scales: Optional[Sequence[torch.Tensor]] = None, seed: int = 0) -> None:
+               exp_avg_sq_scales: Optional[Sequence[torch.Tensor]] = None, seed: int = 0,
+               indices: Optional[Sequence[int]] = None) -> None:
     """One AdamW step over lists of tensors on one device, in place, without synchronising::
 
         m = b1 m + (1 - b1) g      v = b2 v + (1 - b2) g^2      p = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
@@ -272,7 +273,8 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
     them share memory; ``grads`` of the same type, or float32.
     Moments are float32, or -- with both scale lists -- 8 bits: ``exp_avgs`` and ``exp_avg_sqs`` then are ``torch.float8_e4m3fn`` codes of ``m`` and of
     ``sqrt(v)``, each times one float32 scale for 256 consecutive elements (``[ceil(numel / 256)]``).  Codes are rounded stochastically by a hash of
-    (``seed``, tensor, step, element), so that the means do not stall between two codes; equal arguments give equal bits.
+    (``seed``, index, step, element), so that the means do not stall between two codes; equal arguments give equal bits.  A tensor's index is its place in
+    the list, or what ``indices`` says: one that keeps it gets the same bits in any list, and tensors of calls with one seed need different ones.
     ``masters``: float32 copies of 16-bit parameters, which are what is updated; the parameters get the rounded values.
 
     ``step`` is this step's number, from 1 on.  For a step captured into a graph, ``step`` is an int64 device tensor of one element that holds the steps done
@@ -331,6 +333,14 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
     where = list(map(_data_ptr, params))
     if len(set(where)) < len(where) and len({w for w, n in zip(where, numels) if n}) < sum(1 for n in numels if n):
         _refuse(True, "a parameter is in the list twice")
+    if indices is not None:
+        try:
+            places = array("q", indices)
+        except (TypeError, OverflowError):
+            places = ()
+        if len(places) != len(params) or min(places) < 0:
+            _refuse(True, f"indices must be {len(params)} integers from 0 on, got {indices!r}")
+        a.indices = places.buffer_info()[0]
     table = array("q", chain.from_iterable(zip(where, at(grads), at(exp_avgs), at(exp_avg_sqs), at(exp_avg_scales), at(exp_avg_sq_scales), at(masters), numels)))
     a.tensors = table.buffer_info()[0]
     # (the launch goes to the tensors' device, which has to be the current one)
@@ -349,7 +359,7 @@ class AdamW(Optimizer):
     ``master_weights``: bfloat16 / float16 parameters get a float32 copy (``master`` in the state) that carries the updates too small for their type.
     ``capturable``: the step counter lives on the device and ``step()`` may be captured into a graph; ``lr`` may then be a float32 device tensor of one
     element; parameters that were captured together share their counter, so eager steps beside the graph have to be for all of them.  A parameter without
-    a gradient is left alone; ``seed`` picks the random rounding of 8-bit moments."""
+    a gradient is left alone; ``seed`` picks the random rounding of 8-bit moments, in which a parameter's index is its place among all the optimizer's."""
 
     def __init__(self, params, lr: Union[float, torch.Tensor] = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2, amsgrad: bool = False, *,
                  state_bits: int = 32, master_weights: bool = False, capturable: bool = False, seed: int = 0):
@@ -415,9 +425,11 @@ class AdamW(Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        behind = 0                                # parameters in front of the group's
         for group in self.param_groups:
-            calls, fresh = {}, {}
-            for p in group["params"]:
+            calls, fresh, first = {}, {}, behind
+            behind += len(group["params"])
+            for index, p in enumerate(group["params"], first):
                 g = p.grad
                 if g is None:
                     continue
@@ -427,7 +439,7 @@ class AdamW(Optimizer):
                 st = self._state_of(p, group, fresh)
                 t = st["step"]
                 calls.setdefault((p.device, p.dtype, g.dtype, "master" in st, t.data_ptr() if group["capturable"] else t, "exp_avg_scale" in st),
-                                 []).append((p, g, st))
+                                 []).append((p, g, st, index))
             if group["capturable"]:
                 idle = {}                         # parameters that sit this step out keep their count
                 for p in group["params"]:
@@ -447,17 +459,17 @@ class AdamW(Optimizer):
                     if t.data_ptr() in counted:
                         _refuse(_capturing(), "run a step() with these gradients' types before capturing one")
                         t = t.clone()
-                        for _, _, st in items:
+                        for _, _, st, _ in items:
                             st["step"] = t
                     counted.add(t.data_ptr())
             for key, items in calls.items():
-                ps, gs, sts = zip(*items)
+                ps, gs, sts, indices = zip(*items)
                 t = sts[0]["step"] if group["capturable"] else sts[0]["step"] + 1
                 more = {k + "s": [st[k] for st in sts] for k in ("exp_avg_scale", "exp_avg_sq_scale") if k in sts[0]}
                 if key[3]:
                     more["masters"] = [st["master"] for st in sts]
                 adamw_step(ps, gs, [st["exp_avg"] for st in sts], [st["exp_avg_sq"] for st in sts], step=t, lr=group["lr"], betas=group["betas"],
-                           eps=group["eps"], weight_decay=group["weight_decay"], seed=group["seed"], **more)
+                           eps=group["eps"], weight_decay=group["weight_decay"], seed=group["seed"], indices=indices, **more)
                 if not group["capturable"]:
                     for st in sts:
                         st["step"] = t

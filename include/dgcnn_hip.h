@@ -32,7 +32,7 @@
 extern "C" {
 #endif
 
-#define DGCNN_ABI_VERSION 21
+#define DGCNN_ABI_VERSION 22
 
 /* error codes */
 #define DGCNN_OK            0
@@ -351,7 +351,8 @@ int dgcnn_adam_step(float* params, float* grads, float* exp_avg, float* exp_avg_
  * A tensor is `numel` dense elements of param_dtype; grad is of grad_dtype: the same, or fp32.
  * state_bits 32: exp_avg = m, exp_avg_sq = v, fp32.  state_bits 8: exp_avg and exp_avg_sq hold e4m3 codes of m and of sqrt(v), with one fp32
  * scale for each 256 consecutive elements in exp_avg_scale / exp_avg_sq_scale [ceil(numel/256)]: value = code * scale.  Codes are rounded
- * stochastically from a hash of (seed, first_index + tensor, step, element): equal arguments give equal bits.
+ * stochastically from a hash of (seed, index, step, element), tensor i's index being indices[i], or first_index + i where indices is NULL: equal arguments
+ * give equal bits, and a tensor that keeps its index keeps them whatever else is in the list.
  * master (fp32, for 16-bit parameters; all tensors of a call or none): the parameter's full-precision copy, which is what is updated; param
  * gets its rounded value.
  * step >= 1 is this step's number; or step_dev points to a device counter of the steps done so far, which the call increments (for
@@ -368,6 +369,7 @@ typedef struct dgcnn_adamw_args {
   uint64_t seed; int64_t first_index;
   int32_t param_dtype, grad_dtype, state_bits, count;
   const dgcnn_adamw_tensor* tensors;      /* host */
+  const int64_t* indices;                 /* host, [count], or NULL (ABI v22) */
 } dgcnn_adamw_args;
 int dgcnn_adamw_step(const dgcnn_adamw_args* args, dgcnn_stream_t stream);
 
