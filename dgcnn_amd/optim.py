@@ -412,6 +412,8 @@ class AdamW(Optimizer):
         for k, p in zip(saved, mine):
             for name, v in state_dict["state"].get(k, {}).items():
                 if isinstance(v, torch.Tensor):
+                    if name in ("exp_avg", "exp_avg_sq") and v.is_floating_point() and v.dtype.itemsize > 1:
+                        v = v.float()            # (torch holds the moments of 16-bit parameters in 16 bits)
                     if name != "step" and v.shape == p.shape and _layout(v) != _layout(p):
                         if v.dtype.itemsize == 1:
                             raise ValueError("the 8-bit state of a parameter of another memory layout: its blocks are other elements")

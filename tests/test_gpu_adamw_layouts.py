@@ -100,3 +100,23 @@ def test_lists_of_other_shapes_are_refused():
     for lists in ((p, short, ok, ok), (p, ok, short, ok), (p, ok, ok, short)):
         with pytest.raises(_lib.DgcnnError):
             optim.adamw_step(*([t] for t in lists), step=1)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_state_of_torchs_adamw_over_16_bit_parameters_loads(dtype):
+    """torch holds the moments in the parameter's type: they are widened, which is exact"""
+    p = torch.nn.Parameter(torch.linspace(-1, 1, 50).to(dtype).to("cuda"))
+    q = torch.nn.Parameter(p.detach().clone())
+    a, b = torch.optim.AdamW([p], lr=1e-2, foreach=False), optim.AdamW([q], lr=1e-2)
+    g = torch.linspace(1, 2, 50).to(dtype).to("cuda")
+    p.grad = g
+    a.step()
+    b.load_state_dict(a.state_dict())
+    for name in ("exp_avg", "exp_avg_sq"):
+        assert b.state[q][name].dtype == torch.float32 and torch.equal(b.state[q][name].cpu(), a.state[p][name].float().cpu())
+    m = b.state[q]["exp_avg"].cpu().double()
+    q.grad = g
+    b.step()
+    want = 0.9 * m + 0.1 * g.cpu().double()
+    assert b.state[q]["step"] == 2 and ((b.state[q]["exp_avg"].cpu().double() - want).abs() <= 4 * 2.0 ** -24 * want.abs()).all()
