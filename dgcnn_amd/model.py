@@ -81,6 +81,12 @@ def _batch_size_of(data) -> int:
 # Every model's forward tags start somewhere else in the 31-bit range: a workspace is uninitialised memory, and an error word that another
 # model's batch left there must not read as one of this model's.
 _MODELS = itertools.count()
+
+
+def _first_tag() -> int:
+    return next(_MODELS) * 0x9E3779B1 % 0x7FFFFFFE
+
+
 _WS_BYTES = {}      # (N, E, B, F, C) -> dgcnn_workspace_bytes: a pure function of the dimensions, memoised (one ctypes call per step otherwise)
 
 
@@ -170,7 +176,12 @@ class Model(nn.Module):
         self._last_ws = None
         self._last_dims = None
         self._last_flat_grad = None
-        self._epoch = next(_MODELS) * 0x9E3779B1 % 0x7FFFFFFE
+        self._epoch = _first_tag()
+
+    def __setstate__(self, state):
+        """a copy (``copy.deepcopy``, an unpickled module) starts its own tags; the last forward's workspace stays the original's"""
+        super().__setstate__(state)
+        self.__dict__.update(_epoch=_first_tag(), _last_ws=None, _last_dims=None)
 
     # ---- flat parameter buffer ---------------------------------------------------------
     def _param_list(self) -> List[nn.Parameter]:
