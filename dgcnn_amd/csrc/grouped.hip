@@ -118,16 +118,15 @@ typedef short gl_s16x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t gl_u32x4 __attribute__((ext_vector_type(4)));
 
 // G = 16 or 4 bytes of every lane, from base (uniform) + off, to LDS at (uniform) dst + G * lane, without passing through registers.  In assembly because the
-// compiler would wait for every such load before the next LDS read of any kind, i.e. never have one in flight; no register but m0 (which nothing else in
-// these kernels uses) is written, the waits
-// are gl_barrier's.
+// compiler would wait for every such load before the next LDS read of any kind, i.e. never have one in flight; the LDS address is an
+// operand in m0, so that the compiler knows of it (one wait state lies between a write of m0 and such a load); no register is written, the waits are gl_barrier's.
 template <int G> __device__ __forceinline__ void gl_to_lds(const char* base, uint32_t off, char* dst) {
 #ifdef DG_EMU
   for (int i = 0; i < G / 4; ++i) reinterpret_cast<uint32_t*>(dst + G * (threadIdx.x & 63))[i] = reinterpret_cast<const uint32_t*>(base + off)[i];
 #else
   const uint32_t at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)dst);
-  if constexpr (G == 16) asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" :: "s"(at), "v"(off), "s"(base) : "memory");
-  else asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" :: "s"(at), "v"(off), "s"(base) : "memory");
+  if constexpr (G == 16) asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" :: "{m0}"(at), "v"(off), "s"(base) : "memory");
+  else asm volatile("s_nop 0\n\tglobal_load_lds_dword %1, %2" :: "{m0}"(at), "v"(off), "s"(base) : "memory");
 #endif
 }
 // the same from an address of each lane's own
@@ -136,8 +135,8 @@ template <int G> __device__ __forceinline__ void gl_to_lds(const char* src, char
   gl_to_lds<G>(src, 0, dst);
 #else
   const uint32_t at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)dst);
-  if constexpr (G == 16) asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" :: "s"(at), "v"(src) : "memory");
-  else asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" :: "s"(at), "v"(src) : "memory");
+  if constexpr (G == 16) asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, off" :: "{m0}"(at), "v"(src) : "memory");
+  else asm volatile("s_nop 0\n\tglobal_load_lds_dword %1, off" :: "{m0}"(at), "v"(src) : "memory");
 #endif
 }
 template <class T> __device__ __forceinline__ T* gl_uniform(T* p) {      // (the same in every lane: into scalar registers)

@@ -28,3 +28,10 @@ def test_no_script_runs_a_build_without_barriers():
             if os.path.isfile(path):
                 text = open(path, errors="replace").read().lower()
                 assert "nobar" not in text and not re.search(r"-d\w*no_\w*(barrier|wait)", text), path
+
+
+def test_no_assembly_writes_m0_behind_the_compilers_back():
+    """m0 is reserved: a clobber of it is not honoured, so its value goes in as an operand ("{m0}") or not at all"""
+    for path in glob.glob(os.path.join(ROOT, "dgcnn_amd", "csrc", "*.h*")):
+        for n, line in enumerate(open(path), 1):
+            assert not re.search(r"\bs_\w+ m0\b", line), f"{path}:{n}"
