@@ -247,16 +247,15 @@ def _dense(t) -> bool:
     return True
 
 
-def _check_list(name, ts, params, numels, device, dtypes) -> torch.dtype:
-    """Every tensor of one of `dtypes`, as large and laid out as its parameter (or, for scales, `numels` contiguous elements); the type."""
+def _check_list(name, ts, like, numels, device, dtypes) -> torch.dtype:
+    """Every tensor of one of `dtypes`, with `numels` elements, laid out as those of `like` (True: contiguous; None: no matter); the type."""
     # (a few C loops over the whole list; the tensors are looked at one by one only to say which it is)
     kinds = set(map(_get_dtype, ts))
     if len(ts) == len(numels) and len(kinds) == 1 and kinds <= dtypes and set(map(_get_device, ts)) == device and list(map(_numel, ts)) == numels and \
-            (all(map(_is_contiguous, ts)) and (params is None or all(map(_is_contiguous, params)))
-             or params is not None and all(_layout(t) == _layout(p) for t, p in zip(ts, params))):
+            (like is None or (all(map(_is_contiguous, ts)) if like is True else all(_layout(t) == _layout(p) for t, p in zip(ts, like)))):
         return kinds.pop()
     raise _lib.DgcnnError(f"{name} must be {len(numels)} tensors of one type ({', '.join(sorted(map(str, dtypes)))}) on one device, "
-                          + (f"contiguous with one element for each {STATE_BLOCK} of the parameter" if params is None else "with their parameters' sizes and strides")
+                          + (f"contiguous with one element for each {STATE_BLOCK} of the parameter" if name.endswith("scales") else "with their parameters' sizes and strides")
                           + f"; got {len(ts)}: " + ", ".join(f"{t.dtype} {tuple(t.shape)} {t.stride()} on {t.device}" for t in list(ts)[:4]))
 
 
@@ -286,24 +285,25 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
     if not p0.is_cuda:
         _refuse(True, "dgcnn_amd.optim.adamw_step runs only on an AMD GPU through libdgcnn_hip.so; got a CPU tensor")
     numels, device = list(map(_numel, params)), {p0.get_device()}
-    kind = _check_list("params", params, params, numels, device, _DTYPES.keys())
-    if not all(map(_is_contiguous, params)) and not all(map(_dense, params)):
+    kind = _check_list("params", params, None, numels, device, _DTYPES.keys())
+    like = all(map(_is_contiguous, params)) or params
+    if like is params and not all(map(_dense, params)):
         _refuse(True, "parameters must be dense tensors: contiguous in some order of their dimensions")
     bits = 32 if exp_avg_scales is None else 8
     if (exp_avg_scales is None) != (exp_avg_sq_scales is None):
         _refuse(True, "8-bit moments need both exp_avg_scales and exp_avg_sq_scales")
-    gkind = _check_list("grads", grads, params, numels, device, {kind, torch.float32})
+    gkind = _check_list("grads", grads, like, numels, device, {kind, torch.float32})
     state = {torch.float32} if bits == 32 else {torch.float8_e4m3fn}
-    _check_list("exp_avgs", exp_avgs, params, numels, device, state)
-    _check_list("exp_avg_sqs", exp_avg_sqs, params, numels, device, state)
+    _check_list("exp_avgs", exp_avgs, like, numels, device, state)
+    _check_list("exp_avg_sqs", exp_avg_sqs, like, numels, device, state)
     if bits == 8:
         blocks = [-(-n // STATE_BLOCK) for n in numels]
-        _check_list("exp_avg_scales", exp_avg_scales, None, blocks, device, {torch.float32})
-        _check_list("exp_avg_sq_scales", exp_avg_sq_scales, None, blocks, device, {torch.float32})
+        _check_list("exp_avg_scales", exp_avg_scales, True, blocks, device, {torch.float32})
+        _check_list("exp_avg_sq_scales", exp_avg_sq_scales, True, blocks, device, {torch.float32})
     if masters is not None:
         if kind == torch.float32:
             _refuse(True, "masters are for bfloat16 and float16 parameters")
-        _check_list("masters", masters, params, numels, device, {torch.float32})
+        _check_list("masters", masters, like, numels, device, {torch.float32})
     if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0 and eps >= 0.0):
         _refuse(True, f"betas must lie in [0, 1) and eps must not be negative, got {betas}, {eps}")
 
