@@ -340,7 +340,8 @@ int dgcnn_adam_step(float* params, float* grads, float* exp_avg, float* exp_avg_
 
 /* ------------------------------------------------------------------------------------
  * (ABI v21) Operators of wider networks on the same batches: products grouped by type, group norm with an activation, AdamW over many
- * tensors.  Element types are run-time values; sums, statistics and moments are fp32, every result is rounded to its type once.
+ * tensors.  Element types are run-time values; sums, statistics and moments are fp32, every result is rounded to its type once.  Tensors lie at multiples of
+ * their elements' size, workspaces at multiples of 16 bytes.
  * ---------------------------------------------------------------------------------- */
 #define DGCNN_F32  0
 #define DGCNN_BF16 1
