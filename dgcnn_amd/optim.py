@@ -435,7 +435,8 @@ class AdamW(Optimizer):
                 g = p.grad
                 if g is None:
                     continue
-                _refuse(g.is_sparse, "dgcnn_amd.optim.AdamW takes dense gradients")
+                if g.is_sparse:
+                    _refuse(True, "dgcnn_amd.optim.AdamW takes dense gradients")
                 if g.stride() != p.stride() and _layout(g) != _layout(p) and _dense(p):
                     g = torch.empty_like(p, dtype=g.dtype).copy_(g)
                 st = self._state_of(p, group, fresh)
@@ -470,8 +471,10 @@ class AdamW(Optimizer):
                 more = {k + "s": [st[k] for st in sts] for k in ("exp_avg_scale", "exp_avg_sq_scale") if k in sts[0]}
                 if key[3]:
                     more["masters"] = [st["master"] for st in sts]
+                if key[5]:
+                    more["indices"] = indices
                 adamw_step(ps, gs, [st["exp_avg"] for st in sts], [st["exp_avg_sq"] for st in sts], step=t, lr=group["lr"], betas=group["betas"],
-                           eps=group["eps"], weight_decay=group["weight_decay"], seed=group["seed"], indices=indices, **more)
+                           eps=group["eps"], weight_decay=group["weight_decay"], seed=group["seed"], **more)
                 if not group["capturable"]:
                     for st in sts:
                         st["step"] = t
