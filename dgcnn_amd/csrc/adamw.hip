@@ -16,7 +16,7 @@
 // NaN and infinities are coded as NaN and leave the block's scale to its finite elements.
 //
 // Measured (MI355X; a 1 GiB copy reaches 5.2 TB/s): 200 M fp32 elements in 40 tensors 1034 us, 5.4 TB/s; 24 M bf16 ones with fp32 copies and moments in 60 tensors (two
-// launches) 140 us, 4.8 TB/s; 200 M bf16 ones with 8-bit moments 490 us, 4.1 TB/s, held back by the arithmetic of decoding, scaling, hashing and encoding
+// launches) 140 us, 4.8 TB/s; 200 M bf16 ones with 8-bit moments 490 us (under a profiler 514 to 751), 4.1 TB/s, held back by the arithmetic of decoding, scaling, hashing and encoding
 // two codes an element; 16 tensors of 52 K elements together 5.4 us, a launch's own time.
 // The operation sequence is fixed (no contraction): a step's result does not depend on alignment, on the list a tensor is in, or on the launch (with 8-bit
 // moments: as long as the tensor keeps its index).

@@ -6,8 +6,10 @@
 
 Rows are the nodes of a :class:`dgcnn_amd.Batch` (or edges, messages, pixels); ``ptr`` says where each graph's rows begin, as
 :func:`graph_ptr` returns it.  fp32, bf16 and fp16; sums and statistics in fp32.  Everything runs on the current stream of the tensors' device through
-``libdgcnn_hip.so`` without synchronising, forward and backward may be captured into a graph, and equal inputs give equal bits.  As in the rest of the
-package there is no CPU fallback: CPU tensors raise :class:`dgcnn_amd._lib.DgcnnError`.
+``libdgcnn_hip.so`` without synchronising, and equal inputs at equally aligned addresses give equal bits.  Forward and backward may be captured into a graph; as
+with torch's own operators, no eager autograd graph of the same leaves may be alive then (drop its outputs first: its leaves' nodes belong to the eager
+stream).  As in the rest of the package there is no CPU fallback: CPU tensors raise :class:`dgcnn_amd._lib.DgcnnError`.  Derivatives are first ones in reverse mode;
+forward-mode tangents and function transforms raise.
 """
 from __future__ import annotations
 

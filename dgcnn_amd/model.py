@@ -79,7 +79,7 @@ def _batch_size_of(data) -> int:
 
 
 # Every model's forward tags start somewhere else in the 31-bit range: a workspace is uninitialised memory, and an error word that another
-# model's batch left there must not read as one of this model's.
+# model's batch left there should not read as one of this model's (the ranges meet only after millions of forward calls).
 _MODELS = itertools.count()
 
 
